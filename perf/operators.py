@@ -248,6 +248,7 @@ def _plain_logprobs(s):
         g, ge = s["grad_logprobs"][:, None], s["grad_entropy"][:, None]
         one = torch.zeros_like(x).scatter_(1, at, known[:, None].float())
         dx = torch.where(known[:, None], g, 0.0) * (one - p) - ge * (plogp + p * entropy[:, None])
+        dx = torch.where(empty, 0.0, dx)                  # a row whose mask leaves nothing has no gradient
         out.append((dx / _TEMPERATURE).to(logits.dtype))
     return out
 
