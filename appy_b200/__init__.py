@@ -24,7 +24,20 @@ import textwrap
 from . import dispatcher
 from .frontend.static_rewrite import RUNTIME_NAME, rewrite_function_source
 
-__all__ = ["jit", "prange", "range", "vidx", "to_gpu", "to_cpu", "shader", "cpu_shader", "set_default_options"]
+__all__ = ["jit", "prange", "range", "vidx", "to_gpu", "to_cpu", "shader", "cpu_shader", "set_default_options",
+           "embedding", "embedding_grad", "gated_scan", "gated_scan_grad", "token_logprobs", "token_logprobs_grad"]
+
+_OPERATORS = frozenset(__all__[-6:])
+
+
+def __getattr__(name):
+    """The language-model operators (operators.py) need torch, which is imported with the first of them."""
+    if name in _OPERATORS:
+        from . import operators
+        globals().update({n: getattr(operators, n) for n in _OPERATORS})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
 
 _builtin_range = range
 

@@ -83,6 +83,23 @@ SIGNATURES = {
     "appy_spmm_csr_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                     C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int,
                                     C.c_void_p]),
+    "appy_embedding": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64,
+                                 C.c_float, C.c_void_p, C.c_int64, C.c_void_p]),
+    "appy_embedding_grad_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
+    "appy_embedding_grad": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_int64,
+                                      C.c_int64, C.c_float, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_void_p,
+                                      C.c_size_t, C.c_void_p]),
+    "appy_gated_scan": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64] * 2 + [C.c_int, C.c_void_p, C.c_int, C.c_int64,
+                                  C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
+                                  C.c_int, C.c_void_p]),
+    "appy_gated_scan_grad": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64] * 4 + [C.c_int, C.c_void_p, C.c_int,
+                                       C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p] +
+                             [C.c_void_p, C.c_int64, C.c_int64] * 2 + [C.c_void_p, C.c_int, C.c_void_p]),
+    "appy_token_logprobs": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int,
+                                      C.c_float, C.c_int] + [C.c_void_p] * 6),
+    "appy_token_logprobs_grad": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int,
+                                           C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                           C.c_void_p, C.c_int64, C.c_void_p]),
 }
 
 

@@ -18,7 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libappy_sm100.so")
 STAMP = os.path.join(HERE, "libappy_sm100.stamp")
 
-SOURCES = ["appy_shim.cu", "appy_prebuilt.cu", "appy_noalloc.cu"]
+SOURCES = ["appy_shim.cu", "appy_prebuilt.cu", "appy_noalloc.cu", "appy_embedding.cu", "appy_gated_scan.cu",
+           "appy_token_logprobs.cu"]
 
 
 def _nvcc() -> str:
@@ -35,6 +36,7 @@ def _sources() -> list[str]:
 def _digest() -> str:
     h = hashlib.sha256()
     files = _sources() + [os.path.join(HERE, "..", "include", "appy_sm100.h")]
+    files += sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh"))
     tdir = os.path.join(CSRC, "templates")
     files += sorted(os.path.join(tdir, f) for f in os.listdir(tdir))
     for f in files:
@@ -54,7 +56,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     cmd = [
         _nvcc(), "-shared", "-Xcompiler", "-fPIC", "-O3", "-std=c++17", "-lineinfo",
         "-gencode", "arch=compute_100a,code=sm_100a",
-        "-Xptxas", "-v" if verbose else "-O3",
+        "-Xptxas", "-v" if verbose else "-O3", "--threads", "0",
         "-o", LIB, *_sources(),
         "-L" + os.path.join(cuda_home, "lib64"), "-lnvrtc",
         "-Xlinker", "-rpath," + os.path.join(cuda_home, "lib64"),

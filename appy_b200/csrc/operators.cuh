@@ -1,0 +1,140 @@
+// Shared by the language-model operators (appy_embedding.cu, appy_gated_scan.cu, appy_token_logprobs.cu): element
+// types and their conversion to float32, in which every operator computes, and the host-side checks and launch
+// helpers of their C entry points.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+
+#include "../../include/appy_sm100.h"
+#include "templates/appy_device.cuh"
+
+void appy_note_launch();
+int appy_fail_cuda(cudaError_t e, const char* what);
+int appy_fail_arg(const char* what);
+
+namespace appy_op {
+
+typedef __nv_bfloat16 bf16;
+typedef __half f16;
+
+APPY_DEV float to_f32(float v) { return v; }
+APPY_DEV float to_f32(f16 v) { return __half2float(v); }
+APPY_DEV float to_f32(bf16 v) { return __bfloat162float(v); }
+// one rounding to nearest-even, the only one between the float32 arithmetic of an operator and its result
+template <class T> APPY_DEV T from_f32(float v);
+template <> APPY_DEV float from_f32<float>(float v) { return v; }
+template <> APPY_DEV f16 from_f32<f16>(float v) { return __float2half_rn(v); }
+template <> APPY_DEV bf16 from_f32<bf16>(float v) { return __float2bfloat16_rn(v); }
+
+// V elements as one 2..32-byte word, moved as raw bits and converted in registers
+struct __align__(16) Raw32 { uint4 a, b; };
+template <int BYTES> struct Raw { typedef typename appy_raw<BYTES>::type type; };
+template <> struct Raw<32> { typedef Raw32 type; };
+template <class T, int V> struct Pack {
+  typename Raw<sizeof(T) * V>::type raw;
+  union Bits {                                   // the same bits as elements
+    typename Raw<sizeof(T) * V>::type raw;
+    unsigned short h[sizeof(T) * V / 2];
+    unsigned w[(sizeof(T) * V + 3) / 4];
+    APPY_DEV Bits() {}
+  };
+};
+template <class R> APPY_DEV R ld_raw_cs(const R* p) { return __ldcs(p); }
+APPY_DEV Raw32 ld_raw_cs(const Raw32* p) { return {__ldcs(&p->a), __ldcs(&p->b)}; }
+template <class R> APPY_DEV R ld_raw_nc(const R* p) { return __ldg(p); }
+APPY_DEV Raw32 ld_raw_nc(const Raw32* p) { return {__ldg(&p->a), __ldg(&p->b)}; }
+template <class R> APPY_DEV void st_raw_cs(R* p, const R& v) { __stcs(p, v); }
+APPY_DEV void st_raw_cs(Raw32* p, const Raw32& v) { __stcs(&p->a, v.a); __stcs(&p->b, v.b); }
+
+template <class T, int V> APPY_DEV Pack<T, V> ld_stream(const T* p) {        // read once: evict-first
+  return {ld_raw_cs(reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p))};
+}
+template <class T, int V> APPY_DEV Pack<T, V> ld_keep(const T* p) {          // read again soon, never written here
+  return {ld_raw_nc(reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p))};
+}
+template <class T, int V> APPY_DEV Pack<T, V> ld_plain(const T* p) {         // this kernel may also write there
+  return {*reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p)};
+}
+template <class T, int V> APPY_DEV void st_stream(T* p, Pack<T, V> v) {
+  st_raw_cs(reinterpret_cast<typename Raw<sizeof(T) * V>::type*>(p), v.raw);
+}
+template <class T, int V> APPY_DEV void st_plain(T* p, Pack<T, V> v) {
+  *reinterpret_cast<typename Raw<sizeof(T) * V>::type*>(p) = v.raw;
+}
+template <class T, int V> APPY_DEV Pack<T, V> zero_pack() {
+  typename Pack<T, V>::Bits u;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) * V / 2); ++i) u.h[i] = 0;
+  return {u.raw};
+}
+template <class T, int V> APPY_DEV void unpack(Pack<T, V> k, float (&f)[V]) {
+  typename Pack<T, V>::Bits u;
+  u.raw = k.raw;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (sizeof(T) == 4) {
+      f[i] = __uint_as_float(u.w[i]);
+    } else {
+      T t;
+      memcpy(&t, &u.h[i], 2);
+      f[i] = to_f32(t);
+    }
+  }
+}
+template <class T, int V> APPY_DEV Pack<T, V> pack(const float (&f)[V]) {
+  typename Pack<T, V>::Bits u;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (sizeof(T) == 4) {
+      u.w[i] = __float_as_uint(f[i]);
+    } else {
+      const T t = from_f32<T>(f[i]);
+      memcpy(&u.h[i], &t, 2);
+    }
+  }
+  return {u.raw};
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+inline int sm_count() {
+  static int known[16] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return 148;
+  if (!known[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    known[dev] = n;
+  }
+  return known[dev];
+}
+inline int finish(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return appy_fail_cuda(e, what);
+  appy_note_launch();
+  return APPY_OK;
+}
+inline int fail_named(const char* fn, const char* what) {
+  char text[256];
+  snprintf(text, sizeof text, "%s: %s", fn, what);
+  return appy_fail_arg(text);
+}
+inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline int element_size(int dtype) { return dtype == APPY_F32 ? 4 : (dtype == APPY_F16 || dtype == APPY_BF16) ? 2 : 0; }
+
+}  // namespace appy_op
+
+// Runs `...` with `T` standing for the element type that `dtype` names.
+#define APPY_OP_DTYPE(dtype, ...)                                          \
+  [&]() -> int {                                                           \
+    if ((dtype) == APPY_F32) { typedef float T; __VA_ARGS__ }              \
+    if ((dtype) == APPY_F16) { typedef appy_op::f16 T; __VA_ARGS__ }       \
+    typedef appy_op::bf16 T;                                               \
+    __VA_ARGS__                                                            \
+  }()

@@ -182,7 +182,7 @@ int appy_p2p_destroy(void* ctx);
  * combining launches of this context: it starts at 1 and grows by one per launch that uses the
  * mailboxes (this call or a `combine="p2p"` kernel), identically on all ranks. */
 enum { APPY_OP_ADD = 0, APPY_OP_MUL = 1, APPY_OP_MAX = 2, APPY_OP_MIN = 3 };
-enum { APPY_F32 = 0, APPY_F64 = 1, APPY_I32 = 2, APPY_I64 = 3 };
+enum { APPY_F32 = 0, APPY_F64 = 1, APPY_I32 = 2, APPY_I64 = 3, APPY_F16 = 4, APPY_BF16 = 5 };
 int appy_p2p_combine(void* ctx, uint64_t seq, int op, int dtype, void* dvalues, int count, void* stream);
 /* Split-phase form of the exchange: kernels generated with `combine="p2p", defer=True` end like a
  * single-GPU reduction (every CTA stores its partial); one warp at the start of the next such kernel folds
@@ -228,6 +228,64 @@ int appy_gemv_f32(float alpha, const float* dA, int64_t lda, const float* dx, fl
 int appy_spmm_csr_f32(const float* ddata, const int32_t* dindptr, const int32_t* dindices,
                       const float* dB, int64_t ldb, float* dC, int64_t ldc, int64_t row_lo,
                       int64_t row_hi, int ncols, void* stream);
+
+/* ---- language-model operators --------------------------------------------
+ * No counterpart in the reference.  Three operators whose loops the loop templates cannot express: a store whose
+ * row repeats (embedding gradient), a scalar carried along a loop (recurrence), a reduction that carries pairs and
+ * rescales itself (log probabilities).  Element types: dtype is APPY_F32, APPY_F16 or APPY_BF16; arithmetic is
+ * float32, each result is rounded once.  Device pointers of the current device; asynchronous on `stream`; nothing
+ * is allocated, so every call may be captured into a CUDA graph, and calls on different streams share nothing but
+ * what the caller passes to both.  Leading dimensions and strides count elements; rows that start on 16-byte
+ * boundaries (8 for the 16-bit types of the recurrence) and have such widths are moved in packs.  Results do not
+ * depend on scheduling: the same call gives the same bits. */
+
+/* out[n,:] = scale * weight[tokens[n],:] for n < tokens; a token outside [0, rows) gives a row of zeros. */
+int appy_embedding(const void* dweight, int dtype, int64_t ldw, int64_t rows, int64_t width, const void* dtokens,
+                   int token_dtype /* APPY_I32 or APPY_I64 */, int64_t n, float scale, void* dout, int64_t ldo,
+                   void* stream);
+/* out[v,:] = scale * sum of grad[n,:] over all n with tokens[n] == v, for v < rows; with accumulate != 0 the sum is
+ * added to out, and rows without tokens are left as they are.  Tokens outside [0, rows) are dropped.  The sum of a
+ * row runs in float32 over its positions sorted.  out_dtype is dtype or APPY_F32.  `dworkspace` holds at least
+ * appy_embedding_grad_bytes(...) bytes, aligned to 256; its contents before and after do not matter. */
+int appy_embedding_grad_bytes(int64_t n, int64_t rows, int64_t width, size_t* bytes);
+int appy_embedding_grad(const void* dgrad, int dtype, int64_t ldg, const void* dtokens, int token_dtype, int64_t n,
+                        int64_t rows, int64_t width, float scale, int accumulate, void* dout, int out_dtype,
+                        int64_t ldo, void* dworkspace, size_t workspace_bytes, void* stream);
+
+/* Gated linear recurrence of each channel: with f = sigmoid(gate), h[t] = f[t] * h[t-1] + (1 - f[t]) * x[t],
+ * h[-1] = initial (NULL: zeros), last = the state behind the last token (NULL: not wanted; may be `initial`).
+ * Element (sequence s, token t, channel c) of x is dx[s * x_seq + t * x_row + c].  doffsets == NULL: every sequence
+ * has `tokens` tokens.  Otherwise the sequences are packed: doffsets holds sequences + 1 positions (APPY_I32 or
+ * APPY_I64, not decreasing), sequence s is rows [offsets[s], offsets[s+1]) of `tokens` rows in all, the *_seq strides
+ * are not used, positions outside [0, tokens] count as the nearest inside; rows of no sequence are left as they are,
+ * or set to zero with fill != 0.  initial and last are float32 [sequences][width]. */
+int appy_gated_scan(const void* dx, int64_t x_seq, int64_t x_row, const void* dgate, int64_t gate_seq,
+                    int64_t gate_row, int dtype, const void* doffsets, int offsets_dtype, int64_t sequences,
+                    int64_t tokens, int64_t width, const float* dinitial, void* dh, int64_t h_seq, int64_t h_row,
+                    float* dlast, int fill, void* stream);
+/* Its gradient: dh is the recurrence's result, ddh the gradient with respect to it (NULL: zeros), dgrad_last that with
+ * respect to the last state (NULL: zeros); results are the gradients of x, gate and the initial state (NULL: not wanted). */
+int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const void* dx, int64_t x_seq,
+                         int64_t x_row, const void* dgate, int64_t gate_seq, int64_t gate_row, const void* dh,
+                         int64_t h_seq, int64_t h_row, int dtype, const void* doffsets, int offsets_dtype,
+                         int64_t sequences, int64_t tokens, int64_t width, const float* dinitial,
+                         const float* dgrad_last, void* dgrad_x, int64_t gx_seq, int64_t gx_row, void* dgrad_gate,
+                         int64_t gg_seq, int64_t gg_row, float* dgrad_initial, int fill, void* stream);
+
+/* Rows of `cols` logits, z = logits / temperature (in [1e-4, 1e4]): logprobs[n] = log softmax(z)[tokens[n]] (0 for a
+ * token outside [0, cols)), entropy[n] of the row's distribution, stats[n] = {maximum, log2 of the sum, entropy} for
+ * the gradient, and the `top` (0..32, at most cols) largest logits of the row, largest first, equal ones by index:
+ * their log probabilities and indices (top_tokens has the tokens' type).  Logits of -inf have no share; a row of
+ * nothing else has log probability -inf and entropy 0.  A row with NaN or +inf gives NaN. */
+int appy_token_logprobs(const void* dlogits, int dtype, int64_t ld, int64_t rows, int64_t cols, const void* dtokens,
+                        int token_dtype, float temperature, int top, float* dlogprobs, float* dentropy,
+                        float* dstats, float* dtop_logprobs, void* dtop_tokens, void* stream);
+/* Gradient of the logits for the gradients of logprobs and entropy (either may be NULL; strides in elements, 0 for
+ * one value for all rows).  A row of -inf only gets zeros.  dout may be dlogits (with ldo == ld). */
+int appy_token_logprobs_grad(const void* dlogits, int dtype, int64_t ld, int64_t rows, int64_t cols,
+                             const void* dtokens, int token_dtype, float temperature, const float* dstats,
+                             const float* dgrad_logprobs, int64_t grad_logprobs_stride, const float* dgrad_entropy,
+                             int64_t grad_entropy_stride, void* dout, int64_t ldo, void* stream);
 
 /* ---- gather ceilings (measurement aids; no counterpart in the reference) ----
  * What the memory system delivers for the gathers of the two sparse kernels alone, so that their times can
