@@ -47,7 +47,7 @@ struct ScanArgs {
   const void* offsets;       // NULL: every sequence has `tokens` tokens
   bool wide, fill;
   i64 sequences, tokens, width;
-  int tiles, cluster;
+  int tiles;
 };
 
 APPY_DEV i64 offset_at(const ScanArgs& a, i64 s) {
@@ -65,16 +65,64 @@ template <class T, int V> APPY_DEV void clear_rows(const Rows& r, i64 lo, i64 hi
   for (i64 t = lo + sub; t < hi; t += subs) st_stream<T, V>(row_ptr<T>(r, 0, 0, t, col), zero_pack<T, V>());
 }
 
+// What a thread reads of one step: LT tokens of V channels of each of NA arrays (gate, x; gradient: also dh and h of
+// the token before).  Packs go through a ring of `S` stages in shared memory by cp.async, S - 1 steps ahead; a thread
+// reads back only what it copied itself, so the ring needs no barrier.  Elements of 2 bytes, which cp.async cannot
+// move, are loaded into registers one step ahead instead (S = 1).
+template <class T, int V, int LT, int NA, int S> struct Feed {
+  typedef typename Raw<sizeof(T) * V>::type R;
+  static constexpr int kBytes = S > 1 ? S * NA * LT * kBlock * (int)sizeof(R) : 0;
+  const char* from[NA];      // this thread's first row of the next step to fetch
+  i64 row[NA], step[NA];     // bytes from one token to the next in walking order, and from one step to the next
+  R held[S > 1 ? 1 : NA][S > 1 ? 1 : LT];
+  R* ring;
+
+  APPY_DEV void start(int a, const T* p, i64 row_bytes, i64 step_tokens) {
+    from[a] = reinterpret_cast<const char*>(p);
+    row[a] = row_bytes;
+    step[a] = row_bytes * step_tokens;
+  }
+  // rows 0 .. n[a]-1 of the step are there for array a
+  APPY_DEV void fetch(int stage, const int (&n)[NA]) {
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+      const int lim = n[a];
+#pragma unroll
+      for (int j = 0; j < LT; ++j) {
+        const R* src = reinterpret_cast<const R*>(from[a] + j * row[a]);
+        if constexpr (S > 1) {
+          const unsigned dst = (unsigned)__cvta_generic_to_shared(ring + ((stage * NA + a) * LT + j) * kBlock + threadIdx.x);
+          if (j < lim) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(sizeof(R)) : "memory");
+        } else {
+          if (j < lim) held[a][j] = ld_raw_cs(src);
+        }
+      }
+      from[a] += step[a];
+    }
+    if constexpr (S > 1) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  APPY_DEV void arrived() {
+    if constexpr (S > 1) asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+  }
+  APPY_DEV void get(int stage, int a, int j, float (&f)[V]) const {
+    Pack<T, V> k;
+    if constexpr (S > 1) k.raw = ring[((stage * NA + a) * LT + j) * kBlock + threadIdx.x];
+    else k.raw = held[a][j];
+    unpack<T, V>(k, f);
+  }
+};
+
 // V channels per thread, CP threads along the channels, LT tokens per thread, C blocks per cluster.
-template <class T, int V, int LT, int C, bool BACK>
+template <class T, int V, int LT, int S, int C, bool BACK>
 __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
-  constexpr int CP = V == 1 ? 32 : 16, CH = CP * V, SUBS = kBlock / CP, PER_WARP = 32 / CP, L = SUBS * LT;
-  __shared__ __align__(16) float warp_a[2][kWarps][CH], warp_b[2][kWarps][CH];
-  __shared__ __align__(16) float block_a[C > 1 ? 2 : 1][C][CH], block_b[C > 1 ? 2 : 1][C][CH], enter[C > 1 ? 2 : 1][CH];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = tid / CP;
+  constexpr int CP = V == 1 ? 32 : 16, CH = CP * V, SUBS = kBlock / CP, PER_WARP = 32 / CP, L = SUBS * LT, NA = BACK ? 4 : 2;
+  extern __shared__ __align__(16) unsigned char ring_memory[];
+  __shared__ __align__(16) float warp_a[kWarps][CH], warp_b[kWarps][CH], enter[kWarps][CH];
+  __shared__ float block_a[C > 1 ? 2 : 1][C][CH], block_b[C > 1 ? 2 : 1][C][CH];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = tid / CP, pc = (tid % CP) * V;
   const int rank = C > 1 ? blockIdx.x % C : 0;
   const i64 unit = blockIdx.x / C, seq = unit / a.tiles;
-  const i64 chan0 = (unit % a.tiles) * CH, col = chan0 + (tid % CP) * V;
+  const i64 chan0 = (unit % a.tiles) * CH, col = chan0 + pc;
   const bool live = col < a.width;
   i64 first = 0, len = a.tokens, seq_at = seq;
   if (a.offsets) {
@@ -93,78 +141,84 @@ __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
       }
     }
   }
-  // the state that walks along: one block keeps it in every thread for its channels, a cluster in one thread per
-  // channel of every block
-  const float* const start = BACK ? a.dlast : a.initial;
-  float carry[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) carry[v] = 0.f;
-  if (start) {
-    if (C == 1) {
-      if (live) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = start[seq * a.width + col + v];
-      }
-    } else if (tid < CH && chan0 + tid < a.width) {
-      carry[0] = start[seq * a.width + chan0 + tid];
-    }
-  }
+  const bool owner = tid < CH && chan0 + tid < a.width;      // one thread per channel carries the state along
+  float carry = 0.f;
+  if (owner && (BACK ? a.dlast : a.initial)) carry = (BACK ? a.dlast : a.initial)[seq * a.width + chan0 + tid];
   const i64 steps = (len + (i64)L * C - 1) / ((i64)L * C);
-  if (C > 1) cg::this_cluster().sync();            // every block of the cluster runs before its memory is written
+  // this thread's run in the first step, in walking order (backwards for the gradient)
+  const i64 tau0 = (i64)rank * L + sub * LT, t0 = BACK ? len - 1 - tau0 : tau0;
+  const int dir = BACK ? -1 : 1;
+  Feed<T, V, LT, NA, S> feed;
+  feed.ring = reinterpret_cast<typename Feed<T, V, LT, NA, S>::R*>(ring_memory);
+  feed.start(0, row_ptr<const T>(a.gate, seq_at, first, t0, col), dir * a.gate.row * (i64)sizeof(T), (i64)L * C);
+  feed.start(1, row_ptr<const T>(a.x, seq_at, first, t0, col), dir * a.x.row * (i64)sizeof(T), (i64)L * C);
+  if constexpr (BACK) {
+    feed.start(2, row_ptr<const T>(a.dh, seq_at, first, t0, col), dir * a.dh.row * (i64)sizeof(T), (i64)L * C);
+    feed.start(3, row_ptr<const T>(a.h, seq_at, first, t0 - 1, col), dir * a.h.row * (i64)sizeof(T), (i64)L * C);
+  }
+  char* to = reinterpret_cast<char*>(row_ptr<T>(BACK ? a.dx : a.h, seq_at, first, t0, col));
+  char* to_gate = BACK ? reinterpret_cast<char*>(row_ptr<T>(a.dgate, seq_at, first, t0, col)) : nullptr;
+  const i64 to_row = dir * (BACK ? a.dx.row : a.h.row) * (i64)sizeof(T), gate_row = dir * a.dgate.row * (i64)sizeof(T);
+  auto rows_left = [&](i64 k, i64 of) {                      // rows of this thread's run in step k that lie in [.., of)
+    const i64 n = live ? of - (k * L * C + tau0) : 0;
+    return n > LT ? LT : n < 0 ? 0 : (int)n;
+  };
+  auto fetch = [&](int to_stage, i64 k) {
+    const int n = rows_left(k, len);
+    if constexpr (BACK) feed.fetch(to_stage, {n, n, a.dh.base ? n : 0, rows_left(k, len - 1)});      // the first token has none before it
+    else feed.fetch(to_stage, {n, n});
+  };
+  for (int k = 0; k < (S > 1 ? S - 1 : 1); ++k) fetch(k, k);
+  if (C > 1) cg::this_cluster().sync();                      // every block of the cluster runs before its memory is written
+  int stage = 0;
   for (i64 k = 0; k < steps; ++k) {
-    const int buf = (int)(k & 1);
-    const i64 tau0 = (k * C + rank) * L + (i64)sub * LT;      // the run in walking order
+    const int n = rows_left(k, len);
+    if constexpr (S > 1) {
+      fetch(stage == 0 ? S - 1 : stage - 1, k + S - 1);
+      feed.arrived();
+    }
     float f[LT][V], u[LT][V];                      // forward: gate and (1 - gate) * x; gradient: gate and dh
     float in[BACK ? LT : 1][V], w[BACK ? LT : 1][V];          // gradient: 1 - gate and (h[t-1] - x) * gate * (1 - gate)
-    {
-      Pack<T, V> xr[LT], gr[LT], hr[BACK ? LT : 1], dr[BACK ? LT : 1];
 #pragma unroll
-      for (int j = 0; j < LT; ++j) {
-        const i64 tau = tau0 + j, t = BACK ? len - 1 - tau : tau;
-        const bool on = live && tau < len;
-        xr[j] = gr[j] = zero_pack<T, V>();
-        if (BACK) hr[j] = dr[j] = zero_pack<T, V>();
-        if (on) {
-          gr[j] = ld_stream<T, V>(row_ptr<const T>(a.gate, seq_at, first, t, col));
-          xr[j] = ld_stream<T, V>(row_ptr<const T>(a.x, seq_at, first, t, col));
-          if (BACK) {
-            if (a.dh.base) dr[j] = ld_stream<T, V>(row_ptr<const T>(a.dh, seq_at, first, t, col));
-            if (t > 0) hr[j] = ld_stream<T, V>(row_ptr<const T>(a.h, seq_at, first, t - 1, col));
-          }
+    for (int j = 0; j < LT; ++j) {
+      float g[V], x[V];
+      feed.get(stage, 0, j, g);
+      feed.get(stage, 1, j, x);
+      if constexpr (!BACK) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float i;
+          sigmoid_pair(g[v], f[j][v], i);
+          u[j][v] = i * x[v];
         }
-      }
+      } else {
+        float hp[V];
+        feed.get(stage, 2, j, u[j]);
+        feed.get(stage, 3, j, hp);
+        if (!a.dh.base) {
 #pragma unroll
-      for (int j = 0; j < LT; ++j) {
-        const i64 tau = tau0 + j;
-        const bool on = live && tau < len;
-        float x[V], g[V];
-        unpack<T, V>(xr[j], x);
-        unpack<T, V>(gr[j], g);
-        if (!BACK) {
+          for (int v = 0; v < V; ++v) u[j][v] = 0.f;
+        }
+        if (k * L * C + tau0 + j == len - 1 && live) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            float i;
-            sigmoid_pair(g[v], f[j][v], i);
-            u[j][v] = i * x[v];
-            if (!on) f[j][v] = 1.f, u[j][v] = 0.f;
-          }
-        } else {
-          float hp[V];
-          unpack<T, V>(hr[j], hp);
-          unpack<T, V>(dr[j], u[j]);
-          if (on && tau == len - 1 && a.initial) {
+          for (int v = 0; v < V; ++v) hp[v] = a.initial ? a.initial[seq * a.width + col + v] : 0.f;
+        }
 #pragma unroll
-            for (int v = 0; v < V; ++v) hp[v] = a.initial[seq * a.width + col + v];
-          }
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            sigmoid_pair(g[v], f[j][v], in[j][v]);
-            w[j][v] = (hp[v] - x[v]) * (f[j][v] * in[j][v]);
-            if (!on) f[j][v] = 1.f, u[j][v] = 0.f;
-          }
+        for (int v = 0; v < V; ++v) {
+          sigmoid_pair(g[v], f[j][v], in[j][v]);
+          w[j][v] = (hp[v] - x[v]) * (f[j][v] * in[j][v]);
         }
       }
     }
+    if (n < LT) {                                  // tokens past the end change nothing
+#pragma unroll
+      for (int j = 0; j < LT; ++j) {
+        if (j < n) continue;
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[j][v] = 1.f, u[j][v] = 0.f;
+      }
+    }
+    if constexpr (S == 1) fetch(0, k + 1);
     // this thread's run as one map
     float A[V], B[V];
 #pragma unroll
@@ -194,31 +248,20 @@ __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
       }
     }
     if (lane >= 32 - CP) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        warp_a[buf][warp][(tid % CP) * V + v] = A[v];
-        warp_b[buf][warp][(tid % CP) * V + v] = B[v];
-      }
+      st_plain<float, V>(&warp_a[warp][pc], pack<float, V>(A));
+      st_plain<float, V>(&warp_b[warp][pc], pack<float, V>(B));
     }
     __syncthreads();
-    float s[V];                                    // state before this warp's runs
-    if (C == 1) {
-#pragma unroll
-      for (int q = 0; q < kWarps; ++q) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (q == warp) s[v] = carry[v];
-          carry[v] = warp_a[buf][q][(tid % CP) * V + v] * carry[v] + warp_b[buf][q][(tid % CP) * V + v];
-        }
-      }
-    } else {
+    // the channels' threads join the warps' maps (in a cluster first the blocks') and leave each warp its state
+    if constexpr (C > 1) {
       cg::cluster_group cluster = cg::this_cluster();
+      const int buf = (int)(k & 1);
       if (tid < CH) {
         float ba = 1.f, bb = 0.f;
 #pragma unroll
         for (int q = 0; q < kWarps; ++q) {
-          bb = warp_a[buf][q][tid] * bb + warp_b[buf][q][tid];
-          ba *= warp_a[buf][q][tid];
+          bb = warp_a[q][tid] * bb + warp_b[q][tid];
+          ba *= warp_a[q][tid];
         }
 #pragma unroll
         for (int r = 0; r < C; ++r) {
@@ -228,29 +271,36 @@ __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
       }
       cluster.sync();
       if (tid < CH) {
+        float s = 0.f;
 #pragma unroll
         for (int r = 0; r < C; ++r) {
-          if (r == rank) enter[buf][tid] = carry[0];
-          carry[0] = block_a[buf][r][tid] * carry[0] + block_b[buf][r][tid];
+          if (r == rank) s = carry;
+          carry = block_a[buf][r][tid] * carry + block_b[buf][r][tid];
+        }
+#pragma unroll
+        for (int q = 0; q < kWarps; ++q) {
+          enter[q][tid] = s;
+          s = warp_a[q][tid] * s + warp_b[q][tid];
         }
       }
-      __syncthreads();
+    } else if (tid < CH) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[v] = enter[buf][(tid % CP) * V + v];
-      for (int q = 0; q < warp; ++q) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) s[v] = warp_a[buf][q][(tid % CP) * V + v] * s[v] + warp_b[buf][q][(tid % CP) * V + v];
+      for (int q = 0; q < kWarps; ++q) {
+        enter[q][tid] = carry;
+        carry = warp_a[q][tid] * carry + warp_b[q][tid];
       }
     }
+    __syncthreads();
+    float s[V];
+    unpack<float, V>(ld_plain<float, V>(&enter[warp][pc]), s);
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] = ea[v] * s[v] + eb[v];
 #pragma unroll
     for (int j = 0; j < LT; ++j) {
-      const i64 tau = tau0 + j, t = BACK ? len - 1 - tau : tau;
       float o[V], og[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (!BACK) {
+        if constexpr (!BACK) {
           s[v] = f[j][v] * s[v] + u[j][v];
           o[v] = s[v];
         } else {
@@ -260,30 +310,37 @@ __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
           s[v] = f[j][v] * lam;
         }
       }
-      if (live && tau < len) {
-        st_stream<T, V>(row_ptr<T>(BACK ? a.dx : a.h, seq_at, first, t, col), pack<T, V>(o));
-        if (BACK) st_stream<T, V>(row_ptr<T>(a.dgate, seq_at, first, t, col), pack<T, V>(og));
+      if (j < n) {
+        st_stream<T, V>(reinterpret_cast<T*>(to + j * to_row), pack<T, V>(o));
+        if constexpr (BACK) st_stream<T, V>(reinterpret_cast<T*>(to_gate + j * gate_row), pack<T, V>(og));
       }
     }
+    to += to_row * L * C;
+    if (BACK) to_gate += gate_row * L * C;
+    stage = stage + 1 == S ? 0 : stage + 1;
   }
-  if (!a.final_state) return;
-  if (C == 1) {
-    if (sub == 0 && live) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) a.final_state[seq * a.width + col + v] = carry[v];
-    }
-  } else if (rank == 0 && tid < CH && chan0 + tid < a.width) {
-    a.final_state[seq * a.width + chan0 + tid] = carry[0];
-  }
+  if (a.final_state && owner && rank == 0) a.final_state[seq * a.width + chan0 + tid] = carry;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <class T, int V, int LT, int C, bool BACK> int launch_c(const ScanArgs& a, cudaStream_t s) {
+template <class T, int V, int LT, int S, int C, bool BACK> int launch_c(const ScanArgs& a, cudaStream_t s) {
+  const char* const fn = BACK ? "appy_gated_scan_grad" : "appy_gated_scan";
   const i64 blocks = a.sequences * a.tiles * C;
-  if (blocks > 0x7fffffff) return fail_named(BACK ? "appy_gated_scan_grad" : "appy_gated_scan", "too many sequences for one launch");
+  if (blocks > 0x7fffffff) return fail_named(fn, "too many sequences for one launch");
+  const int dyn = Feed<T, V, LT, BACK ? 4 : 2, S>::kBytes;
+  static bool ready[16] = {false};                 // per instantiation and device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 16 || !ready[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(k_scan<T, V, LT, S, C, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn);
+    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(k_scan<T, V, LT, S, C, BACK>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return appy_fail_cuda(e, "gated scan set-up");
+    if (dev >= 0 && dev < 16) ready[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kBlock);
+  cfg.dynamicSmemBytes = dyn;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -291,7 +348,7 @@ template <class T, int V, int LT, int C, bool BACK> int launch_c(const ScanArgs&
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_scan<T, V, LT, C, BACK>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_scan<T, V, LT, S, C, BACK>, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return appy_fail_cuda(e, "gated scan launch");
@@ -299,20 +356,20 @@ template <class T, int V, int LT, int C, bool BACK> int launch_c(const ScanArgs&
   return finish("gated scan launch");
 }
 
-template <class T, int V, int LT, bool BACK> int launch_scan(ScanArgs a, cudaStream_t s) {
+template <class T, int V, int LT, int S, bool BACK> int launch_scan(ScanArgs a, cudaStream_t s) {
   constexpr int CP = V == 1 ? 32 : 16, CH = CP * V, L = kBlock / CP * LT;
   a.tiles = (int)((a.width + CH - 1) / CH);
   // a cluster of blocks along the tokens while there are too few (sequence, channel tile) pairs for two blocks per
   // SM and the cluster's step is not longer than the tokens
   const i64 units = a.sequences * a.tiles;
   int c = 1;
-  while (c < 8 && units * c < 2 * (i64)sm_count() && (i64)L * c < a.tokens) c *= 2;
-  a.cluster = c;
+  while (c < 16 && units * c < 2 * (i64)sm_count() && (i64)L * c < a.tokens) c *= 2;
   switch (c) {
-    case 1: return launch_c<T, V, LT, 1, BACK>(a, s);
-    case 2: return launch_c<T, V, LT, 2, BACK>(a, s);
-    case 4: return launch_c<T, V, LT, 4, BACK>(a, s);
-    default: return launch_c<T, V, LT, 8, BACK>(a, s);
+    case 1: return launch_c<T, V, LT, S, 1, BACK>(a, s);
+    case 2: return launch_c<T, V, LT, S, 2, BACK>(a, s);
+    case 4: return launch_c<T, V, LT, S, 4, BACK>(a, s);
+    case 8: return launch_c<T, V, LT, S, 8, BACK>(a, s);
+    default: return launch_c<T, V, LT, S, 16, BACK>(a, s);
   }
 }
 
@@ -352,7 +409,7 @@ int appy_gated_scan(const void* dx, int64_t x_seq, int64_t x_row, const void* dg
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int size = element_size(dtype);
   const bool vec = width % 4 == 0 && packs(a.x, 4, size) && packs(a.gate, 4, size) && packs(a.h, 4, size);
-  return APPY_OP_DTYPE(dtype, { return vec ? launch_scan<T, 4, 8, false>(a, s) : launch_scan<T, 1, 16, false>(a, s); });
+  return APPY_OP_DTYPE(dtype, { return vec ? launch_scan<T, 4, sizeof(T) == 4 ? 4 : 8, 3, false>(a, s) : launch_scan<T, 1, 16, sizeof(T) == 4 ? 3 : 1, false>(a, s); });
 }
 
 int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const void* dx, int64_t x_seq, int64_t x_row,
@@ -384,7 +441,7 @@ int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const 
   const int size = element_size(dtype);
   const bool vec = width % 4 == 0 && packs(a.x, 4, size) && packs(a.gate, 4, size) && packs(a.h, 4, size) && packs(a.dh, 4, size) &&
                    packs(a.dx, 4, size) && packs(a.dgate, 4, size);
-  return APPY_OP_DTYPE(dtype, { return vec ? launch_scan<T, 4, 4, true>(a, s) : launch_scan<T, 1, 16, true>(a, s); });
+  return APPY_OP_DTYPE(dtype, { return vec ? launch_scan<T, 4, sizeof(T) == 4 ? 2 : 4, 3, true>(a, s) : launch_scan<T, 1, 8, sizeof(T) == 4 ? 3 : 1, true>(a, s); });
 }
 
 }  // extern "C"
