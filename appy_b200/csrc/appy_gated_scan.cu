@@ -23,14 +23,75 @@ namespace {
 using namespace appy_op;
 namespace cg = cooperative_groups;
 
-const int kBlock = 256, kWarps = kBlock / 32;
+const int kBlock = 128;
 
-// f = sigmoid(g) and 1 - f, each to a few units in the last place whichever is small: both come from
-// exp(-|g|) <= 1, so neither overflows nor cancels.
-APPY_DEV void sigmoid_pair(float g, float& f, float& i) {
-  const float e = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + e), er = e * r;
-  f = g >= 0.f ? r : er;
-  i = g >= 0.f ? er : r;
+// ------------------------------------------------------------------------------------------------ V floats at a time
+// Two float32 of one 64-bit register per instruction where V is even: these kernels issue a dozen operations per
+// element, and products and sums of pairs cost half of that.
+template <int V> struct Vec { u64 p[V / 2]; };
+template <> struct Vec<1> { float p[1]; };
+
+APPY_DEV u64 pair(float lo, float hi) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+APPY_DEV float mul1(float a, float b) { return a * b; }
+APPY_DEV float add1(float a, float b) { return a + b; }
+APPY_DEV float fma1(float a, float b, float c) { return fmaf(a, b, c); }
+APPY_DEV u64 mul1(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+APPY_DEV u64 add1(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+APPY_DEV u64 fma1(u64 a, u64 b, u64 c) { u64 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+template <int V> APPY_DEV Vec<V> vec(const float (&f)[V]) {
+  Vec<V> r;
+  if constexpr (V == 1) {
+    r.p[0] = f[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = pair(f[2 * i], f[2 * i + 1]);
+  }
+  return r;
+}
+template <int V> APPY_DEV Vec<V> all(float x) {
+  float f[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = x;
+  return vec<V>(f);
+}
+template <int V> APPY_DEV void floats(const Vec<V>& a, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = a.p[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) asm("mov.b64 {%0, %1}, %2;" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "l"(a.p[i]));
+  }
+}
+#define APPY_EACH(expr)                                                    \
+  Vec<V> r;                                                                \
+  _Pragma("unroll") for (int i = 0; i < (V == 1 ? 1 : V / 2); ++i) r.p[i] = expr; \
+  return r
+template <int V> APPY_DEV Vec<V> mul(const Vec<V>& a, const Vec<V>& b) { APPY_EACH(mul1(a.p[i], b.p[i])); }
+template <int V> APPY_DEV Vec<V> add(const Vec<V>& a, const Vec<V>& b) { APPY_EACH(add1(a.p[i], b.p[i])); }
+template <int V> APPY_DEV Vec<V> fma(const Vec<V>& a, const Vec<V>& b, const Vec<V>& c) { APPY_EACH(fma1(a.p[i], b.p[i], c.p[i])); }
+#undef APPY_EACH
+
+// f = sigmoid(g) and i = 1 - f, each to a few units in the last place whichever is small: with e = exp(-g),
+// f = 1 / (1 + e) and i = e f.  A gate below -87 counts as -87, so that e stays finite: f is 1.6e-38 there, not less.
+template <int V> APPY_DEV void sigmoid_pair(float (&g)[V], Vec<V>& f, Vec<V>& i) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) asm("max.NaN.f32 %0, %0, %1;" : "+f"(g[v]) : "f"(-87.f));
+  float t[V];
+  floats<V>(mul<V>(vec<V>(g), all<V>(-1.44269504088896341f)), t);
+#pragma unroll
+  for (int v = 0; v < V; ++v) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t[v]));
+  const Vec<V> e = vec<V>(t);
+  float d[V];
+  floats<V>(add<V>(e, all<V>(1.f)), d);
+#pragma unroll
+  for (int v = 0; v < V; ++v) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d[v]));
+  f = vec<V>(d);
+  i = mul<V>(e, f);
 }
 
 struct Rows {                // element (sequence s, token t, channel c) is at base + s * seq + t * row + c
@@ -112,14 +173,39 @@ template <class T, int V, int LT, int NA, int S> struct Feed {
   }
 };
 
-// V channels per thread, CP threads along the channels, LT tokens per thread, C blocks per cluster.
-template <class T, int V, int LT, int S, int C, bool BACK>
-__global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
-  constexpr int CP = V == 1 ? 32 : 16, CH = CP * V, SUBS = kBlock / CP, PER_WARP = 32 / CP, L = SUBS * LT, NA = BACK ? 4 : 2;
+// Maps that the blocks of a cluster hand to one another: every block writes its (A, B) of a channel into the same
+// place of every block's shared memory, where the bytes count towards a barrier; no block waits for stores of another
+// kind.  Two buffers alternate: a block sends step k + 2 only after it has everybody's k + 1, which they send after
+// they have read k.
+template <int C, int CH> struct Exchange {
+  u64 map[2][C][CH];
+  u64 full[2];
+};
+APPY_DEV unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+APPY_DEV unsigned in_block(unsigned address, int rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
+  return r;
+}
+APPY_DEV bool wait_full(unsigned barrier, unsigned parity) {           // false: gave up
+  for (unsigned tries = 0; tries < (1u << 22); ++tries) {          // some tenths of a second
+    unsigned done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
+// V channels per thread, CP threads along the channels, LT tokens per thread, C blocks per cluster, S stages.
+template <class T, int V, int CP, int LT, int S, int C, int MIN_BLOCKS, bool BACK>
+__global__ void __launch_bounds__(kBlock, MIN_BLOCKS) k_scan(ScanArgs a) {
+  constexpr int CH = CP * V, SUBS = kBlock / CP, L = SUBS * LT, NA = BACK ? 4 : 2;
+  static_assert(CH <= kBlock, "one thread per channel carries the state");
   extern __shared__ __align__(16) unsigned char ring_memory[];
-  __shared__ __align__(16) float warp_a[kWarps][CH], warp_b[kWarps][CH], enter[kWarps][CH];
-  __shared__ float block_a[C > 1 ? 2 : 1][C][CH], block_b[C > 1 ? 2 : 1][C][CH];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = tid / CP, pc = (tid % CP) * V;
+  __shared__ __align__(16) float run_a[SUBS][CH], run_b[SUBS][CH], enter[SUBS][CH];
+  __shared__ __align__(16) Exchange<C, (C > 1 ? CH : 1)> exchange;
+  const int tid = threadIdx.x, sub = tid / CP, pc = (tid % CP) * V;
   const int rank = C > 1 ? blockIdx.x % C : 0;
   const i64 unit = blockIdx.x / C, seq = unit / a.tiles;
   const i64 chan0 = (unit % a.tiles) * CH, col = chan0 + pc;
@@ -169,7 +255,11 @@ __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
     else feed.fetch(to_stage, {n, n});
   };
   for (int k = 0; k < (S > 1 ? S - 1 : 1); ++k) fetch(k, k);
-  if (C > 1) cg::this_cluster().sync();                      // every block of the cluster runs before its memory is written
+  if constexpr (C > 1) {                           // every block of the cluster runs, its barriers set up, before it is written to
+    if (tid < 2) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&exchange.full[tid])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    cg::this_cluster().sync();
+  }
   int stage = 0;
   for (i64 k = 0; k < steps; ++k) {
     const int n = rows_left(k, len);
@@ -177,142 +267,102 @@ __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
       fetch(stage == 0 ? S - 1 : stage - 1, k + S - 1);
       feed.arrived();
     }
-    float f[LT][V], u[LT][V];                      // forward: gate and (1 - gate) * x; gradient: gate and dh
-    float in[BACK ? LT : 1][V], w[BACK ? LT : 1][V];          // gradient: 1 - gate and (h[t-1] - x) * gate * (1 - gate)
+    Vec<V> f[LT], u[LT];                           // forward: gate and (1 - gate) * x; gradient: gate and dh
+    Vec<V> in[BACK ? LT : 1], w[BACK ? LT : 1];    // gradient: 1 - gate and (h[t-1] - x) * gate * (1 - gate)
 #pragma unroll
     for (int j = 0; j < LT; ++j) {
       float g[V], x[V];
       feed.get(stage, 0, j, g);
       feed.get(stage, 1, j, x);
+      Vec<V> i;
+      sigmoid_pair<V>(g, f[j], i);
       if constexpr (!BACK) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float i;
-          sigmoid_pair(g[v], f[j][v], i);
-          u[j][v] = i * x[v];
-        }
+        u[j] = mul<V>(i, vec<V>(x));
       } else {
-        float hp[V];
-        feed.get(stage, 2, j, u[j]);
+        float hp[V], d[V];
+        feed.get(stage, 2, j, d);
         feed.get(stage, 3, j, hp);
-        if (!a.dh.base) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) u[j][v] = 0.f;
-        }
+        u[j] = a.dh.base ? vec<V>(d) : all<V>(0.f);
         if (k * L * C + tau0 + j == len - 1 && live) {
 #pragma unroll
           for (int v = 0; v < V; ++v) hp[v] = a.initial ? a.initial[seq * a.width + col + v] : 0.f;
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          sigmoid_pair(g[v], f[j][v], in[j][v]);
-          w[j][v] = (hp[v] - x[v]) * (f[j][v] * in[j][v]);
-        }
+        in[j] = i;
+        w[j] = mul<V>(fma<V>(vec<V>(x), all<V>(-1.f), vec<V>(hp)), mul<V>(f[j], i));
       }
     }
     if (n < LT) {                                  // tokens past the end change nothing
 #pragma unroll
-      for (int j = 0; j < LT; ++j) {
-        if (j < n) continue;
-#pragma unroll
-        for (int v = 0; v < V; ++v) f[j][v] = 1.f, u[j][v] = 0.f;
-      }
+      for (int j = 0; j < LT; ++j)
+        if (j >= n) f[j] = all<V>(1.f), u[j] = all<V>(0.f);
     }
     if constexpr (S == 1) fetch(0, k + 1);
     // this thread's run as one map
-    float A[V], B[V];
+    Vec<V> A = f[0], B = BACK ? mul<V>(f[0], u[0]) : u[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      A[v] = 1.f;
-      B[v] = 0.f;
-#pragma unroll
-      for (int j = 0; j < LT; ++j) {
-        A[v] *= f[j][v];
-        B[v] = BACK ? f[j][v] * (B[v] + u[j][v]) : f[j][v] * B[v] + u[j][v];
-      }
+    for (int j = 1; j < LT; ++j) {
+      A = mul<V>(A, f[j]);
+      B = BACK ? mul<V>(f[j], add<V>(B, u[j])) : fma<V>(f[j], B, u[j]);
     }
-    // a warp holds PER_WARP (1 or 2) runs of its channels; its last lanes publish the warp's map
-    float ea[V], eb[V];                            // map of the runs before this one in the warp
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      ea[v] = 1.f;
-      eb[v] = 0.f;
-      if (PER_WARP == 2) {
-        const float pa = __shfl_up_sync(APPY_FULL_MASK, A[v], CP), pb = __shfl_up_sync(APPY_FULL_MASK, B[v], CP);
-        if (lane >= CP) {
-          ea[v] = pa;
-          eb[v] = pb;
-          B[v] = A[v] * pb + B[v];
-          A[v] *= pa;
-        }
-      }
-    }
-    if (lane >= 32 - CP) {
-      st_plain<float, V>(&warp_a[warp][pc], pack<float, V>(A));
-      st_plain<float, V>(&warp_b[warp][pc], pack<float, V>(B));
-    }
+    float o[V];
+    floats<V>(A, o);
+    st_plain<float, V>(&run_a[sub][pc], pack<float, V>(o));
+    floats<V>(B, o);
+    st_plain<float, V>(&run_b[sub][pc], pack<float, V>(o));
     __syncthreads();
-    // the channels' threads join the warps' maps (in a cluster first the blocks') and leave each warp its state
-    if constexpr (C > 1) {
-      cg::cluster_group cluster = cg::this_cluster();
-      const int buf = (int)(k & 1);
-      if (tid < CH) {
+    // the channels' threads join the runs' maps (in a cluster first the blocks') and leave each run its state
+    if (tid < CH) {
+      float s = carry;
+      if constexpr (C > 1) {
+        const int buf = (int)(k & 1);
         float ba = 1.f, bb = 0.f;
 #pragma unroll
-        for (int q = 0; q < kWarps; ++q) {
-          bb = warp_a[q][tid] * bb + warp_b[q][tid];
-          ba *= warp_a[q][tid];
+        for (int q = 0; q < SUBS; ++q) {
+          bb = run_a[q][tid] * bb + run_b[q][tid];
+          ba *= run_a[q][tid];
         }
+        const unsigned full = shared_address(&exchange.full[buf]), place = shared_address(&exchange.map[buf][rank][tid]);
+        if (tid == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "n"(C * CH * 8) : "memory");
+        const u64 map = pair(ba, bb);
 #pragma unroll
-        for (int r = 0; r < C; ++r) {
-          cluster.map_shared_rank(&block_a[buf][rank][tid], r)[0] = ba;
-          cluster.map_shared_rank(&block_b[buf][rank][tid], r)[0] = bb;
-        }
-      }
-      cluster.sync();
-      if (tid < CH) {
-        float s = 0.f;
+        for (int r = 0; r < C; ++r)
+          asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(in_block(place, r)), "l"(map),
+                       "r"(in_block(full, r)) : "memory");
+        if (!wait_full(full, (unsigned)(k >> 1) & 1)) carry = __int_as_float(0x7fffffff);      // cannot happen; shows as NaN
 #pragma unroll
         for (int r = 0; r < C; ++r) {
           if (r == rank) s = carry;
-          carry = block_a[buf][r][tid] * carry + block_b[buf][r][tid];
-        }
-#pragma unroll
-        for (int q = 0; q < kWarps; ++q) {
-          enter[q][tid] = s;
-          s = warp_a[q][tid] * s + warp_b[q][tid];
+          float ra, rb;
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(ra), "=f"(rb) : "l"(exchange.map[buf][r][tid]));
+          carry = ra * carry + rb;
         }
       }
-    } else if (tid < CH) {
 #pragma unroll
-      for (int q = 0; q < kWarps; ++q) {
-        enter[q][tid] = carry;
-        carry = warp_a[q][tid] * carry + warp_b[q][tid];
+      for (int q = 0; q < SUBS; ++q) {
+        enter[q][tid] = s;
+        s = run_a[q][tid] * s + run_b[q][tid];
       }
+      if (C == 1) carry = s;
     }
     __syncthreads();
-    float s[V];
-    unpack<float, V>(ld_plain<float, V>(&enter[warp][pc]), s);
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = ea[v] * s[v] + eb[v];
+    unpack<float, V>(ld_plain<float, V>(&enter[sub][pc]), o);
+    Vec<V> s = vec<V>(o);
 #pragma unroll
     for (int j = 0; j < LT; ++j) {
-      float o[V], og[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if constexpr (!BACK) {
-          s[v] = f[j][v] * s[v] + u[j][v];
-          o[v] = s[v];
-        } else {
-          const float lam = u[j][v] + s[v];
-          o[v] = in[j][v] * lam;
-          og[v] = w[j][v] * lam;
-          s[v] = f[j][v] * lam;
+      if constexpr (!BACK) {
+        s = fma<V>(f[j], s, u[j]);
+        floats<V>(s, o);
+        if (j < n) st_stream<T, V>(reinterpret_cast<T*>(to + j * to_row), pack<T, V>(o));
+      } else {
+        const Vec<V> lam = add<V>(u[j], s);
+        s = mul<V>(f[j], lam);
+        float og[V];
+        floats<V>(mul<V>(in[j], lam), o);
+        floats<V>(mul<V>(w[j], lam), og);
+        if (j < n) {
+          st_stream<T, V>(reinterpret_cast<T*>(to + j * to_row), pack<T, V>(o));
+          st_stream<T, V>(reinterpret_cast<T*>(to_gate + j * gate_row), pack<T, V>(og));
         }
-      }
-      if (j < n) {
-        st_stream<T, V>(reinterpret_cast<T*>(to + j * to_row), pack<T, V>(o));
-        if constexpr (BACK) st_stream<T, V>(reinterpret_cast<T*>(to_gate + j * gate_row), pack<T, V>(og));
       }
     }
     to += to_row * L * C;
@@ -323,8 +373,10 @@ __global__ void __launch_bounds__(kBlock, 2) k_scan(ScanArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <class T, int V, int LT, int S, int C, bool BACK> int launch_c(const ScanArgs& a, cudaStream_t s) {
+template <class T, int V, int CP, int LT, int S, int C, int MIN_BLOCKS, bool BACK> int launch_c(ScanArgs a, cudaStream_t s) {
   const char* const fn = BACK ? "appy_gated_scan_grad" : "appy_gated_scan";
+  const auto kernel = k_scan<T, V, CP, LT, S, C, MIN_BLOCKS, BACK>;
+  a.tiles = (int)((a.width + CP * V - 1) / (CP * V));
   const i64 blocks = a.sequences * a.tiles * C;
   if (blocks > 0x7fffffff) return fail_named(fn, "too many sequences for one launch");
   const int dyn = Feed<T, V, LT, BACK ? 4 : 2, S>::kBytes;
@@ -332,8 +384,8 @@ template <class T, int V, int LT, int S, int C, bool BACK> int launch_c(const Sc
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16 || !ready[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(k_scan<T, V, LT, S, C, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn);
-    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(k_scan<T, V, LT, S, C, BACK>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn);
+    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return appy_fail_cuda(e, "gated scan set-up");
     if (dev >= 0 && dev < 16) ready[dev] = true;
   }
@@ -348,7 +400,7 @@ template <class T, int V, int LT, int S, int C, bool BACK> int launch_c(const Sc
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_scan<T, V, LT, S, C, BACK>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return appy_fail_cuda(e, "gated scan launch");
@@ -356,20 +408,22 @@ template <class T, int V, int LT, int S, int C, bool BACK> int launch_c(const Sc
   return finish("gated scan launch");
 }
 
-template <class T, int V, int LT, int S, bool BACK> int launch_scan(ScanArgs a, cudaStream_t s) {
-  constexpr int CP = V == 1 ? 32 : 16, CH = CP * V, L = kBlock / CP * LT;
-  a.tiles = (int)((a.width + CH - 1) / CH);
-  // a cluster of blocks along the tokens while there are too few (sequence, channel tile) pairs for two blocks per
-  // SM and the cluster's step is not longer than the tokens
-  const i64 units = a.sequences * a.tiles;
+// CP1, S1: threads along the channels and stages of a block on its own, CPC, SC: in a cluster (narrower tiles make
+// more clusters, fewer stages leave room for as many blocks beside the exchange)
+template <class T, int V, int CP1, int CPC, int LT, int S1, int SC, int MIN_BLOCKS, bool BACK> int launch_scan(const ScanArgs& a, cudaStream_t s) {
+  // blocks of their own if they come to two per SM; else clusters along the tokens, up to 16 blocks, as long as the
+  // cluster's step is not longer than the tokens
+  const i64 slots = 2 * (i64)sm_count();
+  if (a.sequences * ((a.width + CP1 * V - 1) / (CP1 * V)) >= slots) return launch_c<T, V, CP1, LT, S1, 1, MIN_BLOCKS, BACK>(a, s);
+  const i64 units = a.sequences * ((a.width + CPC * V - 1) / (CPC * V)), L = kBlock / CPC * LT;
   int c = 1;
-  while (c < 16 && units * c < 2 * (i64)sm_count() && (i64)L * c < a.tokens) c *= 2;
+  while (c < 16 && units * c < 2 * slots && L * c < a.tokens) c *= 2;
   switch (c) {
-    case 1: return launch_c<T, V, LT, S, 1, BACK>(a, s);
-    case 2: return launch_c<T, V, LT, S, 2, BACK>(a, s);
-    case 4: return launch_c<T, V, LT, S, 4, BACK>(a, s);
-    case 8: return launch_c<T, V, LT, S, 8, BACK>(a, s);
-    default: return launch_c<T, V, LT, S, 16, BACK>(a, s);
+    case 1: return launch_c<T, V, CPC, LT, SC, 1, MIN_BLOCKS, BACK>(a, s);
+    case 2: return launch_c<T, V, CPC, LT, SC, 2, MIN_BLOCKS, BACK>(a, s);
+    case 4: return launch_c<T, V, CPC, LT, SC, 4, MIN_BLOCKS, BACK>(a, s);
+    case 8: return launch_c<T, V, CPC, LT, SC, 8, MIN_BLOCKS, BACK>(a, s);
+    default: return launch_c<T, V, CPC, LT, SC, 16, MIN_BLOCKS, BACK>(a, s);
   }
 }
 
@@ -409,7 +463,10 @@ int appy_gated_scan(const void* dx, int64_t x_seq, int64_t x_row, const void* dg
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int size = element_size(dtype);
   const bool vec = width % 4 == 0 && packs(a.x, 4, size) && packs(a.gate, 4, size) && packs(a.h, 4, size);
-  return APPY_OP_DTYPE(dtype, { return vec ? launch_scan<T, 4, sizeof(T) == 4 ? 4 : 8, 3, false>(a, s) : launch_scan<T, 1, 16, sizeof(T) == 4 ? 3 : 1, false>(a, s); });
+  return APPY_OP_DTYPE(dtype, {
+    constexpr bool wide = sizeof(T) == 4;
+    return vec ? launch_scan<T, 4, wide ? 8 : 16, 8, wide ? 4 : 8, 3, 2, 4, false>(a, s) : launch_scan<T, 1, 32, 32, 16, wide ? 3 : 1, wide ? 3 : 1, 4, false>(a, s);
+  });
 }
 
 int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const void* dx, int64_t x_seq, int64_t x_row,
@@ -441,7 +498,10 @@ int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const 
   const int size = element_size(dtype);
   const bool vec = width % 4 == 0 && packs(a.x, 4, size) && packs(a.gate, 4, size) && packs(a.h, 4, size) && packs(a.dh, 4, size) &&
                    packs(a.dx, 4, size) && packs(a.dgate, 4, size);
-  return APPY_OP_DTYPE(dtype, { return vec ? launch_scan<T, 4, sizeof(T) == 4 ? 2 : 4, 3, true>(a, s) : launch_scan<T, 1, 8, sizeof(T) == 4 ? 3 : 1, true>(a, s); });
+  return APPY_OP_DTYPE(dtype, {
+    constexpr bool wide = sizeof(T) == 4;
+    return vec ? launch_scan<T, 4, wide ? 8 : 16, 8, 4, wide ? 2 : 3, 2, wide ? 3 : 4, true>(a, s) : launch_scan<T, 1, 32, 32, 8, wide ? 3 : 1, wide ? 3 : 1, 4, true>(a, s);
+  });
 }
 
 }  // extern "C"
