@@ -12,18 +12,18 @@
 //   mu[t] = f[t] * lam[t],  dx[t] = (1 - f[t]) * lam[t],  dgate[t] = lam[t] * (h[t-1] - x[t]) * f[t] * (1 - f[t]),
 // mu past the last token is the gradient of the last state, mu[0] that of the initial one.
 //
-// A block takes 64 channels (32 where rows do not allow packs) of one sequence and walks along it; with few
-// sequences and channels a cluster of blocks takes neighbouring stretches of tokens in each step, so that the whole
-// machine loads at a time.  States are float32; each result is rounded once.
+// A block takes 64 or 32 channels of one sequence and walks along it; with few sequences and channels a cluster of
+// blocks takes neighbouring stretches of tokens in each step, so that the whole machine loads at a time.  States are float32; each result is rounded once.
 #include <cooperative_groups.h>
+#include <cuda.h>
+
+#include <type_traits>
 
 #include "operators.cuh"
 
 namespace {
 using namespace appy_op;
 namespace cg = cooperative_groups;
-
-const int kBlock = 128;
 
 // ------------------------------------------------------------------------------------------------ V floats at a time
 // Two float32 of one 64-bit register per instruction where V is even: these kernels issue a dozen operations per
@@ -38,9 +38,9 @@ APPY_DEV u64 pair(float lo, float hi) {
 }
 APPY_DEV float mul1(float a, float b) { return a * b; }
 APPY_DEV float add1(float a, float b) { return a + b; }
-APPY_DEV float fma1(float a, float b, float c) { return fmaf(a, b, c); }
 APPY_DEV u64 mul1(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 APPY_DEV u64 add1(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+APPY_DEV float fma1(float a, float b, float c) { return fmaf(a, b, c); }
 APPY_DEV u64 fma1(u64 a, u64 b, u64 c) { u64 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 
 template <int V> APPY_DEV Vec<V> vec(const float (&f)[V]) {
@@ -78,9 +78,25 @@ template <int V> APPY_DEV Vec<V> fma(const Vec<V>& a, const Vec<V>& b, const Vec
 
 // f = sigmoid(g) and i = 1 - f, each to a few units in the last place whichever is small: with e = exp(-g),
 // f = 1 / (1 + e) and i = e f.  A gate below -87 counts as -87, so that e stays finite: f is 1.6e-38 there, not less.
-template <int V> APPY_DEV void sigmoid_pair(float (&g)[V], Vec<V>& f, Vec<V>& i) {
+template <class T, int V> APPY_DEV void bounded_gate(Pack<T, V> k, float (&g)[V]) {
+  if constexpr (sizeof(T) == 2 && V > 1) {         // two at a time, as they came
+    typename Pack<T, V>::Bits u;
+    u.raw = k.raw;
+    const unsigned bound = pack2(-87.f, -87.f, T());
 #pragma unroll
-  for (int v = 0; v < V; ++v) asm("max.NaN.f32 %0, %0, %1;" : "+f"(g[v]) : "f"(-87.f));
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, bf16>::value) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(u.w[i]) : "r"(bound));
+      else asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(u.w[i]) : "r"(bound));
+    }
+    k.raw = u.raw;
+    unpack<T, V>(k, g);
+  } else {
+    unpack<T, V>(k, g);
+#pragma unroll
+    for (int v = 0; v < V; ++v) asm("max.NaN.f32 %0, %0, %1;" : "+f"(g[v]) : "f"(-87.f));
+  }
+}
+template <int V> APPY_DEV void sigmoid_pair(const float (&g)[V], Vec<V>& f, Vec<V>& i) {
   float t[V];
   floats<V>(mul<V>(vec<V>(g), all<V>(-1.44269504088896341f)), t);
 #pragma unroll
@@ -121,91 +137,83 @@ template <class T> APPY_DEV T* row_ptr(const Rows& r, i64 seq, i64 first, i64 t,
 }
 
 // Packed rows that no sequence covers are set to zero where the caller asks for it.
-template <class T, int V> APPY_DEV void clear_rows(const Rows& r, i64 lo, i64 hi, i64 col, bool live, int sub, int subs) {
-  if (!live) return;
-  for (i64 t = lo + sub; t < hi; t += subs) st_stream<T, V>(row_ptr<T>(r, 0, 0, t, col), zero_pack<T, V>());
+template <class T, int V> APPY_DEV void clear_rows(const Rows& r, i64 lo, i64 hi, i64 col, i64 width, int sub, int subs) {
+  for (i64 t = lo + sub; t < hi; t += subs)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (col + v < width) *row_ptr<T>(r, 0, 0, t, col + v) = from_f32<T>(0.f);
 }
 
-// What a thread reads of one step: LT tokens of V channels of each of NA arrays (gate, x; gradient: also dh and h of
-// the token before).  Packs go through a ring of `S` stages in shared memory by cp.async, S - 1 steps ahead; a thread
-// reads back only what it copied itself, so the ring needs no barrier.  Elements of 2 bytes, which cp.async cannot
-// move, are loaded into registers one step ahead instead (S = 1).
-template <class T, int V, int LT, int NA, int S> struct Feed {
-  typedef typename Raw<sizeof(T) * V>::type R;
-  static constexpr int kBytes = S > 1 ? S * NA * LT * kBlock * (int)sizeof(R) : 0;
-  const char* from[NA];      // this thread's first row of the next step to fetch
-  i64 row[NA], step[NA];     // bytes from one token to the next in walking order, and from one step to the next
-  R held[S > 1 ? 1 : NA][S > 1 ? 1 : LT];
-  R* ring;
-
-  APPY_DEV void start(int a, const T* p, i64 row_bytes, i64 step_tokens) {
-    from[a] = reinterpret_cast<const char*>(p);
-    row[a] = row_bytes;
-    step[a] = row_bytes * step_tokens;
-  }
-  // rows 0 .. n[a]-1 of the step are there for array a
-  APPY_DEV void fetch(int stage, const int (&n)[NA]) {
-#pragma unroll
-    for (int a = 0; a < NA; ++a) {
-      const int lim = n[a];
-#pragma unroll
-      for (int j = 0; j < LT; ++j) {
-        const R* src = reinterpret_cast<const R*>(from[a] + j * row[a]);
-        if constexpr (S > 1) {
-          const unsigned dst = (unsigned)__cvta_generic_to_shared(ring + ((stage * NA + a) * LT + j) * kBlock + threadIdx.x);
-          if (j < lim) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(sizeof(R)) : "memory");
-        } else {
-          if (j < lim) held[a][j] = ld_raw_cs(src);
-        }
-      }
-      from[a] += step[a];
-    }
-    if constexpr (S > 1) asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-  APPY_DEV void arrived() {
-    if constexpr (S > 1) asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-  }
-  APPY_DEV void get(int stage, int a, int j, float (&f)[V]) const {
-    Pack<T, V> k;
-    if constexpr (S > 1) k.raw = ring[((stage * NA + a) * LT + j) * kBlock + threadIdx.x];
-    else k.raw = held[a][j];
-    unpack<T, V>(k, f);
-  }
-};
-
-// Maps that the blocks of a cluster hand to one another: every block writes its (A, B) of a channel into the same
-// place of every block's shared memory, where the bytes count towards a barrier; no block waits for stores of another
-// kind.  Two buffers alternate: a block sends step k + 2 only after it has everybody's k + 1, which they send after
-// they have read k.
-template <int C, int CH> struct Exchange {
-  u64 map[2][C][CH];
-  u64 full[2];
-};
 APPY_DEV unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+// The wait suspends the warp for up to a microsecond at a time; false: it gave up after about a second.
+APPY_DEV bool wait_full(unsigned barrier, unsigned parity) {
+  for (unsigned tries = 0; tries < (1u << 20); ++tries) {
+    unsigned done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done) : "r"(barrier), "r"(parity), "r"(1000u) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+APPY_DEV void expect_bytes(unsigned barrier, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
+}
+
+// The arrays that a step reads: gate, x; for the gradient also dh and h of the token before.
+template <int NA> struct Maps { CUtensorMap m[NA]; };
+struct NoMaps {};
+
+// What the blocks of a cluster tell one another about a step.  Each channel has an owner among the blocks: every block
+// sends it the channel's map (A, B) over its stretch of the step, the owner, which also carries the channel's state from
+// step to step, sends every block the state that its stretch begins with.  Both travel as st.async, whose bytes count
+// towards a barrier of the receiver, so no block waits for stores of another kind, and a step costs 2 CH messages per
+// block however large the cluster is (all maps to all blocks were C CH, and the step 3.4 us for C = 16).
+// Two buffers alternate: a channel's map of step k + 2 is sent after its state of step k + 1 has come, which its owner
+// sends after it has read the maps of step k, and its state of step k + 2 after all blocks' maps of step k + 2, which
+// they send after they have read their state of step k.
+template <int C, int CH> struct Exchange {
+  u64 map[2][C][CH / C];
+  float state[2][CH];
+  u64 maps_full[2], states_full[2];
+};
 APPY_DEV unsigned in_block(unsigned address, int rank) {
   unsigned r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
   return r;
 }
-APPY_DEV bool wait_full(unsigned barrier, unsigned parity) {           // false: gave up
-  for (unsigned tries = 0; tries < (1u << 22); ++tries) {          // some tenths of a second
-    unsigned done;
-    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
-    if (done) return true;
-  }
-  return false;
-}
+// V channels per thread, CP threads along the channels, LT tokens per thread, NT threads, C blocks per cluster.
+//
+// Where rows start on 16-byte boundaries, TMA brings the tiles of a step (L tokens of CH channels of each array) into a
+// ring of S stages, some steps ahead (S > 1, V = 4); what lies outside the arrays arrives as zeros.  Elsewhere every
+// thread loads its elements into registers one step ahead (S = 1, V = 1).
+//
+// While the maps of step k + 1 travel (to the other warps; in a cluster to the owners and back), step k is replayed and
+// the maps of step k + 2 are made: a step waits for nobody in the middle, and one barrier per step is enough.
+template <class T, int V, int CP, int LT, int S, int NT, int C, bool BACK> struct Shape {
+  static constexpr int CH = CP * V, SUBS = NT / CP, L = SUBS * LT, NA = BACK ? 4 : 2;
+  struct Shared {
+    T ring[S > 1 ? S : 1][2][S > 1 ? L * CH : 8];                // gate and x; gradient: gate and dh
+    T late[S > 1 && BACK ? S : 1][2][S > 1 && BACK ? L * CH : 8];      // gradient: x and h of the token before
+    float run_a[2][SUBS][CH], run_b[2][SUBS][CH], enter[2][SUBS][CH];
+    Exchange<C, CH> exchange;
+    u64 loaded[S], late_loaded[S];
+  };
+};
 
-// V channels per thread, CP threads along the channels, LT tokens per thread, C blocks per cluster, S stages.
-template <class T, int V, int CP, int LT, int S, int C, int MIN_BLOCKS, bool BACK>
-__global__ void __launch_bounds__(kBlock, MIN_BLOCKS) k_scan(ScanArgs a) {
-  constexpr int CH = CP * V, SUBS = kBlock / CP, L = SUBS * LT, NA = BACK ? 4 : 2;
-  static_assert(CH <= kBlock, "one thread per channel carries the state");
-  extern __shared__ __align__(16) unsigned char ring_memory[];
-  __shared__ __align__(16) float run_a[SUBS][CH], run_b[SUBS][CH], enter[SUBS][CH];
-  __shared__ __align__(16) Exchange<C, (C > 1 ? CH : 1)> exchange;
-  const int tid = threadIdx.x, sub = tid / CP, pc = (tid % CP) * V;
+template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, bool BACK>
+__global__ void __launch_bounds__(NT, MIN_BLOCKS)
+k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 1), Maps<BACK ? 4 : 2>, NoMaps>::type maps) {
+  typedef Shape<T, V, CP, LT, S, NT, C, BACK> Sh;
+  constexpr int CH = Sh::CH, SUBS = Sh::SUBS, L = Sh::L, NA = Sh::NA;
+  // The maps of a step are joined by all threads: a warp takes WC channels, G lanes of it share a channel's runs.
+  constexpr int WC = CH / (NT / 32), G = 32 / WC, PER = SUBS / G;
+  static_assert(G * WC == 32 && PER * G == SUBS, "every run of every channel belongs to one lane");
+  // The gradient needs x and h only when it replays a step; from a ring they are read as late as that.
+  constexpr bool KEEP = !BACK || S == 1;
+  extern __shared__ __align__(128) unsigned char shared_memory[];
+  typename Sh::Shared& sh = *reinterpret_cast<typename Sh::Shared*>(shared_memory);
+  const int tid = threadIdx.x, lane = tid & 31, sub = tid / CP, pc = (tid % CP) * V;
+  const int join_ch = tid / 32 * WC + lane % WC, join_run = lane / WC * PER;
   const int rank = C > 1 ? blockIdx.x % C : 0;
   const i64 unit = blockIdx.x / C, seq = unit / a.tiles;
   const i64 chan0 = (unit % a.tiles) * CH, col = chan0 + pc;
@@ -218,181 +226,390 @@ __global__ void __launch_bounds__(kBlock, MIN_BLOCKS) k_scan(ScanArgs a) {
     seq_at = 0;
     if (a.fill && rank == 0) {
       if (seq == 0) {
-        clear_rows<T, V>(BACK ? a.dx : a.h, 0, first, col, live, sub, SUBS);
-        if (BACK) clear_rows<T, V>(a.dgate, 0, first, col, live, sub, SUBS);
+        clear_rows<T, V>(BACK ? a.dx : a.h, 0, first, col, a.width, sub, SUBS);
+        if (BACK) clear_rows<T, V>(a.dgate, 0, first, col, a.width, sub, SUBS);
       }
       if (seq == a.sequences - 1) {
-        clear_rows<T, V>(BACK ? a.dx : a.h, end, a.tokens, col, live, sub, SUBS);
-        if (BACK) clear_rows<T, V>(a.dgate, end, a.tokens, col, live, sub, SUBS);
+        clear_rows<T, V>(BACK ? a.dx : a.h, end, a.tokens, col, a.width, sub, SUBS);
+        if (BACK) clear_rows<T, V>(a.dgate, end, a.tokens, col, a.width, sub, SUBS);
       }
     }
   }
-  const bool owner = tid < CH && chan0 + tid < a.width;      // one thread per channel carries the state along
+  // The state before the step whose maps are joined next: in a block of its own in all G lanes of a channel, in a
+  // cluster in C threads of the channel's owner.
+  constexpr int OWN = CH / C;
+  const int carry_ch = C == 1 ? join_ch : rank * OWN + tid % OWN;
   float carry = 0.f;
-  if (owner && (BACK ? a.dlast : a.initial)) carry = (BACK ? a.dlast : a.initial)[seq * a.width + chan0 + tid];
+  const float* const start = BACK ? a.dlast : a.initial;
+  if (start && chan0 + carry_ch < a.width) carry = start[seq * a.width + chan0 + carry_ch];
   const i64 steps = (len + (i64)L * C - 1) / ((i64)L * C);
   // this thread's run in the first step, in walking order (backwards for the gradient)
   const i64 tau0 = (i64)rank * L + sub * LT, t0 = BACK ? len - 1 - tau0 : tau0;
-  const int dir = BACK ? -1 : 1;
-  Feed<T, V, LT, NA, S> feed;
-  feed.ring = reinterpret_cast<typename Feed<T, V, LT, NA, S>::R*>(ring_memory);
-  feed.start(0, row_ptr<const T>(a.gate, seq_at, first, t0, col), dir * a.gate.row * (i64)sizeof(T), (i64)L * C);
-  feed.start(1, row_ptr<const T>(a.x, seq_at, first, t0, col), dir * a.x.row * (i64)sizeof(T), (i64)L * C);
-  if constexpr (BACK) {
-    feed.start(2, row_ptr<const T>(a.dh, seq_at, first, t0, col), dir * a.dh.row * (i64)sizeof(T), (i64)L * C);
-    feed.start(3, row_ptr<const T>(a.h, seq_at, first, t0 - 1, col), dir * a.h.row * (i64)sizeof(T), (i64)L * C);
-  }
+  constexpr int dir = BACK ? -1 : 1;
   char* to = reinterpret_cast<char*>(row_ptr<T>(BACK ? a.dx : a.h, seq_at, first, t0, col));
   char* to_gate = BACK ? reinterpret_cast<char*>(row_ptr<T>(a.dgate, seq_at, first, t0, col)) : nullptr;
   const i64 to_row = dir * (BACK ? a.dx.row : a.h.row) * (i64)sizeof(T), gate_row = dir * a.dgate.row * (i64)sizeof(T);
-  auto rows_left = [&](i64 k, i64 of) {                      // rows of this thread's run in step k that lie in [.., of)
+  auto rows_left = [&](i64 k, i64 of) {            // rows of this thread's run in step k that lie in [.., of)
     const i64 n = live ? of - (k * L * C + tau0) : 0;
     return n > LT ? LT : n < 0 ? 0 : (int)n;
   };
-  auto fetch = [&](int to_stage, i64 k) {
-    const int n = rows_left(k, len);
-    if constexpr (BACK) feed.fetch(to_stage, {n, n, a.dh.base ? n : 0, rows_left(k, len - 1)});      // the first token has none before it
-    else feed.fetch(to_stage, {n, n});
+  bool in_time = true;                             // a wait that gave up (which cannot happen) shows as NaN
+
+  // ---- reading: array 0 gate, 1 x, 2 dh, 3 h of the token before
+  Pack<T, V> held[S > 1 ? 1 : NA][S > 1 ? 1 : LT];
+  int make_stage = 0, replay_stage = 0;
+  unsigned make_parity = 0, replay_parity = 0;
+  auto next = [](int& stage, unsigned& parity) {
+    stage = stage + 1 == S ? 0 : stage + 1;
+    if (stage == 0) parity ^= 1;
   };
-  for (int k = 0; k < (S > 1 ? S - 1 : 1); ++k) fetch(k, k);
-  if constexpr (C > 1) {                           // every block of the cluster runs, its barriers set up, before it is written to
-    if (tid < 2) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&exchange.full[tid])) : "memory");
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    cg::this_cluster().sync();
-  }
-  int stage = 0;
-  for (i64 k = 0; k < steps; ++k) {
-    const int n = rows_left(k, len);
+  auto load = [&](u64* loaded, i64 k, auto& ring, int x, int y) {        // two arrays of step k by TMA
+    if (tid != 0 || k >= steps) return;
+    const int stage = (int)(k % S);
+    const unsigned barrier = shared_address(&loaded[stage]);
+    const bool first_too = x != 2 || a.dh.base, second_too = y != 2 || a.dh.base;
+    expect_bytes(barrier, (first_too + second_too) * (unsigned)(L * CH * sizeof(T)));
     if constexpr (S > 1) {
-      fetch(stage == 0 ? S - 1 : stage - 1, k + S - 1);
-      feed.arrived();
+      const i64 base = (k * C + rank) * L, t = first + (BACK ? len - base - L : base);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int array = q ? y : x;
+        if (q ? second_too : first_too)
+          asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                           shared_address(&ring[stage][q][0])),
+                       "l"(&maps.m[array]), "r"((int)chan0), "r"((int)(array == 3 ? t - 1 : t)), "r"((int)seq_at), "r"(barrier)
+                       : "memory");
+      }
     }
-    Vec<V> f[LT], u[LT];                           // forward: gate and (1 - gate) * x; gradient: gate and dh
-    Vec<V> in[BACK ? LT : 1], w[BACK ? LT : 1];    // gradient: 1 - gate and (h[t-1] - x) * gate * (1 - gate)
+  };
+  const T* from[NA];                               // S = 1: this thread's first row of the step to fetch next
+  i64 from_row[NA];
+  if constexpr (S == 1) {
+#pragma unroll
+    for (int x = 0; x < NA; ++x) {
+      const Rows& r = x == 0 ? a.gate : x == 1 ? a.x : x == 2 ? a.dh : a.h;
+      from[x] = row_ptr<const T>(r, seq_at, first, x == 3 ? t0 - 1 : t0, col);
+      from_row[x] = dir * r.row;
+    }
+  }
+  auto fetch = [&](i64 k) {                        // what step k is made from (registers: all of it)
+    if constexpr (S > 1) {
+      load(sh.loaded, k, sh.ring, 0, BACK ? 2 : 1);
+    } else {
+      const int n = rows_left(k, len), n_before = BACK ? rows_left(k, len - 1) : 0;      // the first token has none before it
+#pragma unroll
+      for (int x = 0; x < NA; ++x) {
+        const int lim = x == 3 ? n_before : x == 2 && !a.dh.base ? 0 : n;
+#pragma unroll
+        for (int j = 0; j < LT; ++j)
+          if (j < lim) held[x][j] = ld_stream<T, V>(from[x] + j * from_row[x]);
+        from[x] += from_row[x] * L * C;
+      }
+    }
+  };
+  auto fetch_late = [&](i64 k) {
+    if constexpr (S > 1 && BACK) load(sh.late_loaded, k, sh.late, 1, 3);
+  };
+  const int at_row = BACK ? L - 1 - sub * LT : sub * LT;
+  auto word = [&](const auto& ring, int stage, int q, int x, int j) -> Pack<T, V> {
+    if constexpr (S > 1) return ld_plain<T, V>(&ring[stage][q][(at_row + dir * j) * CH + pc]);
+    else return held[x][j];
+  };
+
+  struct Step {
+    Vec<V> f[LT];                                  // gate
+    Vec<V> i[BACK ? LT : 1];                       // gradient: 1 - gate
+    Vec<V> u[BACK ? 1 : LT];                       // forward: (1 - gate) * x
+    Pack<T, V> dh[BACK ? LT : 1];                  // gradient, as it came
+    Vec<V> w[BACK && KEEP ? LT : 1];               // gradient: h[t-1] - x
+  };
+  auto dh_of = [&](Pack<T, V> word) {
+    float d[V];
+    unpack<T, V>(word, d);
+    return a.dh.base ? vec<V>(d) : all<V>(0.f);
+  };
+  auto difference = [&](int stage, int first_token, int j) {      // h[t-1] - x
+    float x[V], hp[V];
+    unpack<T, V>(word(sh.late, stage, 0, 1, j), x);
+    unpack<T, V>(word(sh.late, stage, 1, NA - 1, j), hp);
+    if (j == first_token) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) hp[v] = a.initial && col + v < a.width ? a.initial[seq * a.width + col + v] : 0.f;
+    }
+    return fma<V>(vec<V>(x), all<V>(-1.f), vec<V>(hp));
+  };
+  // gates and maps of step k
+  auto make = [&](i64 k, Step& st) {
+    const int buf = (int)(k & 1), n = rows_left(k, len), n_before = BACK ? rows_left(k, len - 1) : n;      // one less where the sequence begins
+    if constexpr (S > 1) in_time = in_time && wait_full(shared_address(&sh.loaded[make_stage]), make_parity);
+    Vec<V> u[LT];
 #pragma unroll
     for (int j = 0; j < LT; ++j) {
-      float g[V], x[V];
-      feed.get(stage, 0, j, g);
-      feed.get(stage, 1, j, x);
+      float g[V];
+      bounded_gate<T, V>(word(sh.ring, make_stage, 0, 0, j), g);
       Vec<V> i;
-      sigmoid_pair<V>(g, f[j], i);
-      if constexpr (!BACK) {
-        u[j] = mul<V>(i, vec<V>(x));
+      sigmoid_pair<V>(g, st.f[j], i);
+      if constexpr (BACK) {
+        st.i[j] = i;
+        st.dh[j] = word(sh.ring, make_stage, 1, NA - 2, j);
+        u[j] = dh_of(st.dh[j]);
+        if constexpr (KEEP) st.w[j] = difference(make_stage, n - n_before == 1 ? n_before : -1, j);
       } else {
-        float hp[V], d[V];
-        feed.get(stage, 2, j, d);
-        feed.get(stage, 3, j, hp);
-        u[j] = a.dh.base ? vec<V>(d) : all<V>(0.f);
-        if (k * L * C + tau0 + j == len - 1 && live) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) hp[v] = a.initial ? a.initial[seq * a.width + col + v] : 0.f;
-        }
-        in[j] = i;
-        w[j] = mul<V>(fma<V>(vec<V>(x), all<V>(-1.f), vec<V>(hp)), mul<V>(f[j], i));
+        float x[V];
+        unpack<T, V>(word(sh.ring, make_stage, 1, 1, j), x);
+        u[j] = mul<V>(i, vec<V>(x));
       }
     }
     if (n < LT) {                                  // tokens past the end change nothing
 #pragma unroll
       for (int j = 0; j < LT; ++j)
-        if (j >= n) f[j] = all<V>(1.f), u[j] = all<V>(0.f);
+        if (j >= n) st.f[j] = all<V>(1.f), u[j] = all<V>(0.f);
     }
-    if constexpr (S == 1) fetch(0, k + 1);
-    // this thread's run as one map
-    Vec<V> A = f[0], B = BACK ? mul<V>(f[0], u[0]) : u[0];
+    Vec<V> A = st.f[0], B = BACK ? mul<V>(st.f[0], u[0]) : u[0];
 #pragma unroll
-    for (int j = 1; j < LT; ++j) {
-      A = mul<V>(A, f[j]);
-      B = BACK ? mul<V>(f[j], add<V>(B, u[j])) : fma<V>(f[j], B, u[j]);
+    for (int j = 0; j < LT; ++j) {
+      if constexpr (!BACK) st.u[j] = u[j];
+      if (j == 0) continue;
+      A = mul<V>(A, st.f[j]);
+      B = BACK ? mul<V>(st.f[j], add<V>(B, u[j])) : fma<V>(st.f[j], B, u[j]);
     }
+    next(make_stage, make_parity);
     float o[V];
     floats<V>(A, o);
-    st_plain<float, V>(&run_a[sub][pc], pack<float, V>(o));
+    st_plain<float, V>(&sh.run_a[buf][sub][pc], pack<float, V>(o));
     floats<V>(B, o);
-    st_plain<float, V>(&run_b[sub][pc], pack<float, V>(o));
-    __syncthreads();
-    // the channels' threads join the runs' maps (in a cluster first the blocks') and leave each run its state
-    if (tid < CH) {
-      float s = carry;
-      if constexpr (C > 1) {
-        const int buf = (int)(k & 1);
-        float ba = 1.f, bb = 0.f;
+    st_plain<float, V>(&sh.run_b[buf][sub][pc], pack<float, V>(o));
+  };
+  // joins the maps of step k: this lane's PER runs, the G lanes of the channel (in a cluster the blocks, for which
+  // `send` and `join` come apart), and leaves each run the state it starts from
+  float ma[PER], mb[PER], before_a, before_b;
+  auto send = [&](i64 k) {
+    const int buf = (int)(k & 1);
+    float A = 1.f, B = 0.f;
 #pragma unroll
-        for (int q = 0; q < SUBS; ++q) {
-          bb = run_a[q][tid] * bb + run_b[q][tid];
-          ba *= run_a[q][tid];
-        }
-        const unsigned full = shared_address(&exchange.full[buf]), place = shared_address(&exchange.map[buf][rank][tid]);
-        if (tid == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "n"(C * CH * 8) : "memory");
-        const u64 map = pair(ba, bb);
-#pragma unroll
-        for (int r = 0; r < C; ++r)
-          asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(in_block(place, r)), "l"(map),
-                       "r"(in_block(full, r)) : "memory");
-        if (!wait_full(full, (unsigned)(k >> 1) & 1)) carry = __int_as_float(0x7fffffff);      // cannot happen; shows as NaN
-#pragma unroll
-        for (int r = 0; r < C; ++r) {
-          if (r == rank) s = carry;
-          float ra, rb;
-          asm("mov.b64 {%0, %1}, %2;" : "=f"(ra), "=f"(rb) : "l"(exchange.map[buf][r][tid]));
-          carry = ra * carry + rb;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < SUBS; ++q) {
-        enter[q][tid] = s;
-        s = run_a[q][tid] * s + run_b[q][tid];
-      }
-      if (C == 1) carry = s;
+    for (int q = 0; q < PER; ++q) {
+      ma[q] = sh.run_a[buf][join_run + q][join_ch];
+      mb[q] = sh.run_b[buf][join_run + q][join_ch];
+      B = ma[q] * B + mb[q];
+      A *= ma[q];
     }
-    __syncthreads();
-    unpack<float, V>(ld_plain<float, V>(&enter[sub][pc]), o);
-    Vec<V> s = vec<V>(o);
+#pragma unroll
+    for (int o = WC; o < 32; o *= 2) {
+      const float pa = __shfl_up_sync(APPY_FULL_MASK, A, o), pb = __shfl_up_sync(APPY_FULL_MASK, B, o);
+      if (lane >= o) {
+        B = A * pb + B;
+        A *= pa;
+      }
+    }
+    before_a = 1.f;
+    before_b = 0.f;
+    if constexpr (G > 1) {
+      const float pa = __shfl_up_sync(APPY_FULL_MASK, A, WC), pb = __shfl_up_sync(APPY_FULL_MASK, B, WC);
+      if (lane >= WC) before_a = pa, before_b = pb;
+    }
+    if constexpr (C > 1) {
+      const unsigned full = shared_address(&sh.exchange.maps_full[buf]);
+      if (tid == 0) {
+        expect_bytes(full, CH * 8);
+        expect_bytes(shared_address(&sh.exchange.states_full[buf]), CH * 4);
+      }
+      if (lane >= 32 - WC)                         // the last of a channel's lanes has the block's map
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
+                         in_block(shared_address(&sh.exchange.map[buf][rank][join_ch % OWN]), join_ch / OWN)),
+                     "l"(pair(A, B)), "r"(in_block(full, join_ch / OWN))
+                     : "memory");
+    }
+  };
+  auto answer = [&](i64 k) {                       // the owner's part: thread (channel, block)
+    if (tid >= CH) return;
+    const int buf = (int)(k & 1), ch = tid % OWN, to_rank = tid / OWN;
+    in_time = in_time && wait_full(shared_address(&sh.exchange.maps_full[buf]), (unsigned)(k >> 1) & 1);
+    float s = carry;
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
+      if (r == to_rank) s = carry;
+      float ra, rb;
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(ra), "=f"(rb) : "l"(sh.exchange.map[buf][r][ch]));
+      carry = ra * carry + rb;
+    }
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(
+                     in_block(shared_address(&sh.exchange.state[buf][rank * OWN + ch]), to_rank)),
+                 "r"(__float_as_uint(s)), "r"(in_block(shared_address(&sh.exchange.states_full[buf]), to_rank))
+                 : "memory");
+  };
+  auto join = [&](i64 k) {
+    const int buf = (int)(k & 1);
+    float s = carry;
+    if constexpr (C > 1) {
+      in_time = in_time && wait_full(shared_address(&sh.exchange.states_full[buf]), (unsigned)(k >> 1) & 1);
+      s = sh.exchange.state[buf][join_ch];
+    }
+    s = before_a * s + before_b;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      sh.enter[buf][join_run + q][join_ch] = s;
+      s = ma[q] * s + mb[q];
+    }
+    if constexpr (C == 1) carry = __shfl_sync(APPY_FULL_MASK, s, 32 - WC + lane % WC);
+  };
+  auto replay = [&](i64 k, const Step& st) {
+    const int buf = (int)(k & 1), n = rows_left(k, len), n_before = BACK ? rows_left(k, len - 1) : n;
+    if constexpr (S > 1 && BACK) in_time = in_time && wait_full(shared_address(&sh.late_loaded[replay_stage]), replay_parity);
+    float o[V];
+    unpack<float, V>(ld_plain<float, V>(&sh.enter[buf][sub][pc]), o);
+    Vec<V> state = vec<V>(o);
 #pragma unroll
     for (int j = 0; j < LT; ++j) {
       if constexpr (!BACK) {
-        s = fma<V>(f[j], s, u[j]);
-        floats<V>(s, o);
+        state = fma<V>(st.f[j], state, st.u[j]);
+        floats<V>(state, o);
         if (j < n) st_stream<T, V>(reinterpret_cast<T*>(to + j * to_row), pack<T, V>(o));
       } else {
-        const Vec<V> lam = add<V>(u[j], s);
-        s = mul<V>(f[j], lam);
+        Vec<V> w;
+        if constexpr (KEEP) w = st.w[j];
+        else w = difference(replay_stage, n - n_before == 1 ? n_before : -1, j);
+        const Vec<V> lam = add<V>(dh_of(st.dh[j]), state);
+        state = mul<V>(st.f[j], lam);
         float og[V];
-        floats<V>(mul<V>(in[j], lam), o);
-        floats<V>(mul<V>(w[j], lam), og);
+        const Vec<V> d = mul<V>(st.i[j], lam);
+        floats<V>(d, o);
+        floats<V>(mul<V>(w, mul<V>(st.f[j], d)), og);
         if (j < n) {
           st_stream<T, V>(reinterpret_cast<T*>(to + j * to_row), pack<T, V>(o));
           st_stream<T, V>(reinterpret_cast<T*>(to_gate + j * gate_row), pack<T, V>(og));
         }
       }
     }
+    if constexpr (BACK) next(replay_stage, replay_parity);
     to += to_row * L * C;
     if (BACK) to_gate += gate_row * L * C;
-    stage = stage + 1 == S ? 0 : stage + 1;
+  };
+  if (S > 1 || C > 1) {                            // barriers, before anybody counts on them
+    if (tid < S) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&sh.loaded[tid])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&sh.late_loaded[tid])) : "memory");
+    }
+    if (tid < 2) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&sh.exchange.maps_full[tid])) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&sh.exchange.states_full[tid])) : "memory");
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if constexpr (C > 1) cg::this_cluster().sync();          // every block of the cluster runs before it is written to
+    else __syncthreads();
   }
-  if (a.final_state && owner && rank == 0) a.final_state[seq * a.width + chan0 + tid] = carry;
+  for (int k = 0; k < S; ++k) {
+    fetch(k);
+    fetch_late(k);
+  }
+  if (steps > 0) {
+    Step even, odd;
+    // A stage is free once all threads have done with its step: made it, or, for what comes late, replayed it.
+    auto refill = [&](i64 made) {
+      if constexpr (S > 1) fetch(made + S);
+    };
+    auto advance = [&](i64 k, Step& st) {          // st: step k, then step k + 2
+      const bool more = k + 1 < steps;
+      if (more) send(k + 1);
+      if (C == 1 && more) join(k + 1);
+      replay(k, st);
+      if (C > 1 && more) answer(k + 1);
+      if (k + 2 < steps) {
+        make(k + 2, st);
+        if constexpr (S == 1) fetch(k + 3);
+      }
+      if (C > 1 && more) join(k + 1);
+      __syncthreads();
+      refill(k + 2);
+      fetch_late(k + S);
+    };
+    make(0, even);
+    if constexpr (S == 1) fetch(1);
+    __syncthreads();
+    refill(0);
+    send(0);
+    if constexpr (C > 1) answer(0);
+    if (steps > 1) {
+      make(1, odd);
+      if constexpr (S == 1) fetch(2);
+    }
+    join(0);
+    __syncthreads();
+    refill(1);
+    for (i64 k = 0; k < steps; k += 2) {
+      advance(k, even);
+      if (k + 1 < steps) advance(k + 1, odd);
+    }
+  }
+  if (!in_time) carry = __int_as_float(0x7fffffff);
+  if (a.final_state && (C == 1 ? lane < WC : tid < OWN) && chan0 + carry_ch < a.width) a.final_state[seq * a.width + chan0 + carry_ch] = carry;
+}
+
+// One token of every sequence, the step of a serving loop: no scan, a thread per channel.
+template <class T> __global__ void __launch_bounds__(256) k_scan_token(ScanArgs a) {
+  const i64 i = (i64)blockIdx.x * 256 + threadIdx.x, seq = i / a.width, col = i - seq * a.width;
+  if (seq >= a.sequences) return;
+  float g[1] = {to_f32(*row_ptr<const T>(a.gate, seq, 0, 0, col))};
+  const float x = to_f32(*row_ptr<const T>(a.x, seq, 0, 0, col));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(g[0]) : "f"(-87.f));
+  Vec<1> f, in;
+  sigmoid_pair<1>(g, f, in);
+  const float h = fmaf(f.p[0], a.initial ? a.initial[i] : 0.f, in.p[0] * x);
+  *row_ptr<T>(a.h, seq, 0, 0, col) = from_f32<T>(h);
+  if (a.final_state) a.final_state[i] = h;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <class T, int V, int CP, int LT, int S, int C, int MIN_BLOCKS, bool BACK> int launch_c(ScanArgs a, cudaStream_t s) {
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// The array as (channel, token, sequence), read in boxes of `channels` by `tokens`.
+template <class T> bool encode(CUtensorMap* m, const Rows& r, const ScanArgs& a, int channels, int tokens) {
+  const i64 sequences = a.offsets ? 1 : a.sequences;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.width, (cuuint64_t)a.tokens, (cuuint64_t)sequences};
+  const cuuint64_t strides[2] = {(cuuint64_t)r.row * sizeof(T), (cuuint64_t)(sequences > 1 ? r.seq : r.row) * sizeof(T)};
+  const cuuint32_t box[3] = {(cuuint32_t)channels, (cuuint32_t)tokens, 1}, unit[3] = {1, 1, 1};
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : std::is_same<T, f16>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode_tiled()(m, type, 3, r.base, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+const int kNoTma = -1000;                          // not a status: TMA cannot describe the arrays, read them without it
+
+template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, bool BACK> int launch_c(ScanArgs a, cudaStream_t s) {
+  typedef Shape<T, V, CP, LT, S, NT, C, BACK> Sh;
   const char* const fn = BACK ? "appy_gated_scan_grad" : "appy_gated_scan";
-  const auto kernel = k_scan<T, V, CP, LT, S, C, MIN_BLOCKS, BACK>;
-  a.tiles = (int)((a.width + CP * V - 1) / (CP * V));
+  const auto kernel = k_scan<T, V, CP, LT, S, NT, C, MIN_BLOCKS, BACK>;
+  a.tiles = (int)((a.width + Sh::CH - 1) / Sh::CH);
   const i64 blocks = a.sequences * a.tiles * C;
   if (blocks > 0x7fffffff) return fail_named(fn, "too many sequences for one launch");
-  const int dyn = Feed<T, V, LT, BACK ? 4 : 2, S>::kBytes;
   static bool ready[16] = {false};                 // per instantiation and device
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16 || !ready[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename Sh::Shared));
     if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return appy_fail_cuda(e, "gated scan set-up");
     if (dev >= 0 && dev < 16) ready[dev] = true;
   }
+  typename std::conditional<(S > 1), Maps<BACK ? 4 : 2>, NoMaps>::type maps;
+  if constexpr (S > 1) {
+    const Rows* rows[4] = {&a.gate, &a.x, a.dh.base ? &a.dh : &a.gate, &a.h};
+    for (int x = 0; x < Sh::NA; ++x)
+      if (!encode<T>(&maps.m[x], *rows[x], a, Sh::CH, Sh::L)) return kNoTma;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(kBlock);
-  cfg.dynamicSmemBytes = dyn;
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = sizeof(typename Sh::Shared);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -400,7 +617,7 @@ template <class T, int V, int CP, int LT, int S, int C, int MIN_BLOCKS, bool BAC
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, maps);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return appy_fail_cuda(e, "gated scan launch");
@@ -408,26 +625,70 @@ template <class T, int V, int CP, int LT, int S, int C, int MIN_BLOCKS, bool BAC
   return finish("gated scan launch");
 }
 
-// CP1, S1: threads along the channels and stages of a block on its own, CPC, SC: in a cluster (narrower tiles make
-// more clusters, fewer stages leave room for as many blocks beside the exchange)
-template <class T, int V, int CP1, int CPC, int LT, int S1, int SC, int MIN_BLOCKS, bool BACK> int launch_scan(const ScanArgs& a, cudaStream_t s) {
-  // blocks of their own if they come to two per SM; else clusters along the tokens, up to 16 blocks, as long as the
-  // cluster's step is not longer than the tokens
-  const i64 slots = 2 * (i64)sm_count();
-  if (a.sequences * ((a.width + CP1 * V - 1) / (CP1 * V)) >= slots) return launch_c<T, V, CP1, LT, S1, 1, MIN_BLOCKS, BACK>(a, s);
-  const i64 units = a.sequences * ((a.width + CPC * V - 1) / (CPC * V)), L = kBlock / CPC * LT;
+// Variants, each with the time of the one it was chosen over (B200, bfloat16 unless said, forward / gradient):
+//   many (sequence, 64 channels) pairs, four per SM: 64-channel blocks of 4 tokens per thread, four to an SM
+//     (64 x 512 x 2048: 71 us; 32-channel blocks of 8 tokens per thread 96 us);
+//   fewer: 32-channel blocks, twice as many; forward 8 tokens per thread and two blocks to an SM (8 x 2048 x 2048:
+//     46 us; the first variant 53 us), gradient 4 tokens per thread and four blocks (73 us; the first variant 94 us);
+//   fewer than two 32-channel blocks per SM: clusters along the tokens, as many blocks as keep to two per SM, which
+//     is where all clusters run at once (65536 x 1024: 8 blocks 106 us, 16 blocks 160 us, one block 493 us);
+//     packed sequences, whose lengths are uneven, up to six per SM (37 sequences of 0 to 8000 tokens of 648 float32
+//     channels: two blocks 85 / 153 us, one 85 / 176 us).
+template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t s) {
+  constexpr bool wide = sizeof(T) == 4;
+  constexpr int S = wide || BACK ? 2 : 4, LT = BACK ? 4 : 8;
+  const i64 sms = sm_count(), units = a.sequences * ((a.width + 31) / 32), wide_units = a.sequences * ((a.width + 63) / 64);
+  if (wide_units >= 4 * sms || a.tokens <= 32) return launch_c<T, 4, 16, 4, S, 128, 1, BACK && wide ? 3 : 4, BACK>(a, s);
+  const i64 most = a.offsets ? 12 * sms : 2 * sms;
   int c = 1;
-  while (c < 16 && units * c < 2 * slots && L * c < a.tokens) c *= 2;
+  while (c < 16 && units * 2 * c <= most && (i64)16 * LT * c < a.tokens) c *= 2;
   switch (c) {
-    case 1: return launch_c<T, V, CPC, LT, SC, 1, MIN_BLOCKS, BACK>(a, s);
-    case 2: return launch_c<T, V, CPC, LT, SC, 2, MIN_BLOCKS, BACK>(a, s);
-    case 4: return launch_c<T, V, CPC, LT, SC, 4, MIN_BLOCKS, BACK>(a, s);
-    case 8: return launch_c<T, V, CPC, LT, SC, 8, MIN_BLOCKS, BACK>(a, s);
-    default: return launch_c<T, V, CPC, LT, SC, 16, MIN_BLOCKS, BACK>(a, s);
+    case 1: return launch_c<T, 4, 8, LT, S, 128, 1, BACK ? (wide ? 3 : 4) : 2, BACK>(a, s);
+    case 2: return launch_c<T, 4, 8, LT, S, 128, 2, 2, BACK>(a, s);
+    case 4: return launch_c<T, 4, 8, LT, S, 128, 4, 2, BACK>(a, s);
+    case 8: return launch_c<T, 4, 8, LT, S, 128, 8, 2, BACK>(a, s);
+    default: return launch_c<T, 4, 8, LT, S, 128, 16, 2, BACK>(a, s);
   }
 }
+// Rows that TMA cannot read: the same with direct loads.
+template <class T, bool BACK> int launch_direct(const ScanArgs& a, cudaStream_t s) {
+  constexpr int LT = BACK ? 4 : 8;
+  const i64 sms = sm_count(), units = a.sequences * ((a.width + 31) / 32);
+  int c = 1;
+  while (c < 16 && units * 2 * c <= (a.offsets ? 12 : 4) * sms && (i64)4 * LT * c < a.tokens) c *= 2;
+  switch (c) {
+    case 1: return launch_c<T, 1, 32, LT, 1, 128, 1, 4, BACK>(a, s);
+    case 2: return launch_c<T, 1, 32, LT, 1, 128, 2, 4, BACK>(a, s);
+    case 4: return launch_c<T, 1, 32, LT, 1, 128, 4, 4, BACK>(a, s);
+    case 8: return launch_c<T, 1, 32, LT, 1, 128, 8, 4, BACK>(a, s);
+    default: return launch_c<T, 1, 32, LT, 1, 128, 16, 4, BACK>(a, s);
+  }
+}
+template <class T> int launch_token(const ScanArgs& a, cudaStream_t s) {
+  const i64 blocks = (a.sequences * a.width + 255) / 256;
+  if (blocks > 0x7fffffff) return fail_named("appy_gated_scan", "too many sequences for one launch");
+  k_scan_token<T><<<(unsigned)blocks, 256, 0, s>>>(a);
+  return finish("gated scan launch");
+}
 
-bool packs(const Rows& r, int V, int size) { return !r.base || (r.seq % V == 0 && r.row % V == 0 && aligned(r.base, (size_t)V * size)); }
+// Whether TMA can read, and packs of four can be stored to, this array.
+bool packs(const Rows& r, const ScanArgs& a, int size) {
+  if (!r.base) return true;
+  const i64 v = 16 / size;
+  const bool rows = r.row % v == 0 && r.row >= a.width && r.row < (1ll << 36);
+  const bool seqs = a.offsets || a.sequences == 1 || (r.seq % v == 0 && r.seq > 0 && r.seq < (1ll << 36));
+  return aligned(r.base, 16) && rows && seqs;
+}
+bool packs(const ScanArgs& a, int size) {
+  return a.width % 4 == 0 && a.tokens > 0 && a.tokens < (1ll << 31) && a.sequences < (1ll << 31) && encode_tiled() && packs(a.x, a, size) && packs(a.gate, a, size) &&
+         packs(a.h, a, size) && packs(a.dh, a, size) && packs(a.dx, a, size) && packs(a.dgate, a, size);
+}
+
+template <class T, bool BACK> int launch_scan(const ScanArgs& a, cudaStream_t s) {
+  if (!BACK && !a.offsets && a.tokens == 1) return launch_token<T>(a, s);
+  const int rc = packs(a, sizeof(T)) ? launch_packed<T, BACK>(a, s) : kNoTma;
+  return rc == kNoTma ? launch_direct<T, BACK>(a, s) : rc;
+}
 
 int check_shape(const char* fn, int dtype, const void* offsets, int offsets_dtype, i64 sequences, i64 tokens, i64 width) {
   if (!element_size(dtype)) return fail_named(fn, "dtype must be APPY_F32, APPY_F16 or APPY_BF16");
@@ -461,12 +722,7 @@ int appy_gated_scan(const void* dx, int64_t x_seq, int64_t x_row, const void* dg
   a.tokens = tokens;
   a.width = width;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int size = element_size(dtype);
-  const bool vec = width % 4 == 0 && packs(a.x, 4, size) && packs(a.gate, 4, size) && packs(a.h, 4, size);
-  return APPY_OP_DTYPE(dtype, {
-    constexpr bool wide = sizeof(T) == 4;
-    return vec ? launch_scan<T, 4, wide ? 8 : 16, 8, wide ? 4 : 8, 3, 2, 4, false>(a, s) : launch_scan<T, 1, 32, 32, 16, wide ? 3 : 1, wide ? 3 : 1, 4, false>(a, s);
-  });
+  return APPY_OP_DTYPE(dtype, { return launch_scan<T, false>(a, s); });
 }
 
 int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const void* dx, int64_t x_seq, int64_t x_row,
@@ -495,13 +751,7 @@ int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const 
   a.tokens = tokens;
   a.width = width;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int size = element_size(dtype);
-  const bool vec = width % 4 == 0 && packs(a.x, 4, size) && packs(a.gate, 4, size) && packs(a.h, 4, size) && packs(a.dh, 4, size) &&
-                   packs(a.dx, 4, size) && packs(a.dgate, 4, size);
-  return APPY_OP_DTYPE(dtype, {
-    constexpr bool wide = sizeof(T) == 4;
-    return vec ? launch_scan<T, 4, wide ? 8 : 16, 8, 4, wide ? 2 : 3, 2, wide ? 3 : 4, true>(a, s) : launch_scan<T, 1, 32, 32, 8, wide ? 3 : 1, wide ? 3 : 1, 4, true>(a, s);
-  });
+  return APPY_OP_DTYPE(dtype, { return launch_scan<T, true>(a, s); });
 }
 
 }  // extern "C"

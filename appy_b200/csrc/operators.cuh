@@ -74,30 +74,50 @@ template <class T, int V> APPY_DEV Pack<T, V> zero_pack() {
   for (int i = 0; i < (int)(sizeof(T) * V / 2); ++i) u.h[i] = 0;
   return {u.raw};
 }
+// two 16-bit elements of one register to and from float32
+APPY_DEV void unpack2(unsigned w, float& lo, float& hi, bf16) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xffff0000u);
+}
+APPY_DEV void unpack2(unsigned w, float& lo, float& hi, f16) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.f32.f16 %0, l;\ncvt.f32.f16 %1, h;\n}" : "=f"(lo), "=f"(hi) : "r"(w));
+}
+APPY_DEV unsigned pack2(float lo, float hi, bf16) {
+  unsigned w;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+  return w;
+}
+APPY_DEV unsigned pack2(float lo, float hi, f16) {
+  unsigned w;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+  return w;
+}
 template <class T, int V> APPY_DEV void unpack(Pack<T, V> k, float (&f)[V]) {
   typename Pack<T, V>::Bits u;
   u.raw = k.raw;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (sizeof(T) == 4) {
-      f[i] = __uint_as_float(u.w[i]);
-    } else {
-      T t;
-      memcpy(&t, &u.h[i], 2);
-      f[i] = to_f32(t);
-    }
+    for (int i = 0; i < V; ++i) f[i] = __uint_as_float(u.w[i]);
+  } else if constexpr (V == 1) {
+    T t;
+    memcpy(&t, &u.h[0], 2);
+    f[0] = to_f32(t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) unpack2(u.w[i], f[2 * i], f[2 * i + 1], T());
   }
 }
 template <class T, int V> APPY_DEV Pack<T, V> pack(const float (&f)[V]) {
   typename Pack<T, V>::Bits u;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (sizeof(T) == 4) {
-      u.w[i] = __float_as_uint(f[i]);
-    } else {
-      const T t = from_f32<T>(f[i]);
-      memcpy(&u.h[i], &t, 2);
-    }
+    for (int i = 0; i < V; ++i) u.w[i] = __float_as_uint(f[i]);
+  } else if constexpr (V == 1) {
+    const T t = from_f32<T>(f[0]);
+    memcpy(&u.h[0], &t, 2);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) u.w[i] = pack2(f[2 * i], f[2 * i + 1], T());
   }
   return {u.raw};
 }

@@ -266,7 +266,10 @@ def _sequences(fn, x, offsets):
 def _scan_in(fn, name, t, x):
     if t is not x:
         _like(fn, name, t, x.shape, x.dtype)
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    if t.is_contiguous():
+        return t
+    strides = [stride for stride, size in zip(t.stride(), t.shape) if size > 1]
+    return t.contiguous() if 0 in strides or (t.shape[-1] > 1 and t.stride(-1) != 1) else t
 
 
 def _scan_out(fn, name, t, x):

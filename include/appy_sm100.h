@@ -236,7 +236,7 @@ int appy_spmm_csr_f32(const float* ddata, const int32_t* dindptr, const int32_t*
  * float32, each result is rounded once.  Device pointers of the current device; asynchronous on `stream`; nothing
  * is allocated, so every call may be captured into a CUDA graph, and calls on different streams share nothing but
  * what the caller passes to both.  Leading dimensions and strides count elements; rows that start on 16-byte
- * boundaries (8 for the 16-bit types of the recurrence) and have such widths are moved in packs.  Results do not
+ * boundaries and have such widths are moved in packs.  Results do not
  * depend on scheduling: the same call gives the same bits. */
 
 /* out[n,:] = scale * weight[tokens[n],:] for n < tokens; a token outside [0, rows) gives a row of zeros. */
