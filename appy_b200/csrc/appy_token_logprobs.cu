@@ -25,7 +25,7 @@ namespace {
 using namespace appy_op;
 namespace cg = cooperative_groups;
 
-const int kBlock = 512, kWarps = kBlock / 32, kTopMax = 32, kGroups = 64, kCandidates = 1024;
+const int kTopMax = 32;
 
 APPY_DEV float neg_inf() { return __int_as_float(0xff800000); }
 APPY_DEV float quiet_nan() { return __int_as_float(0x7fffffff); }
@@ -41,7 +41,7 @@ APPY_DEV float max_nan(float a, float b) {               // NaN if either is
 }
 
 // k and a bound: a maximum within +-limit stays within float32 when multiplied by k
-struct Scale { float k, limit, inv_temperature; };
+struct Scale { float k, limit, span, inv_temperature; };      // span: 2^(-span k) is below float32
 
 // d = (x - m) * k.  For a maximum within the limit as one fused multiply-add against the rounded product m * k: that product is a
 // reference like any other, as long as every use of this m has the same one (so it must not be contracted into a
@@ -97,32 +97,136 @@ struct Split {
 
 struct Best { unsigned value; int at; };                 // ordered value and first index of the best pack
 
-template <int V, bool TOP> APPY_DEV void take(const float (&x)[V], int at, Part& p, Best& best, const Scale& s) {
-  float m = x[0];
+// Maximum of a pack (NaN if one is), and the pack with everything below `bound` raised to it; 16-bit types two at a time.
+template <class T, int V> APPY_DEV float pack_max(const Pack<T, V>& k) {
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    typename Pack<T, V>::Bits u;
+    u.raw = k.raw;
+    unsigned m = u.w[0];
 #pragma unroll
-  for (int v = 1; v < V; ++v) m = max_nan(m, x[v]);
-  if (TOP) {
-    const unsigned o = ordered(m);
-    if (o > best.value) best = {o, at};
-  }
-  if (!(m <= p.m)) p = rescaled(p, max_nan(m, p.m), s);      // a NaN stays
-  const Scaled d(p.m, s);
-  if (!d.far) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float t = d.fast(x[v], s), e = exp2_fast(t);
-      p.s += e;
-      p.q = fmaf(e, t, p.q);
+    for (int i = 1; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, bf16>::value) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(u.w[i]));
+      else asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(u.w[i]));
     }
-  } else if (fabsf(p.m) < __int_as_float(0x7f800000)) {
+    float lo, hi;
+    unpack2(m, lo, hi, T());
+    return max_nan(lo, hi);
+  } else {
+    float x[V];
+    unpack<T, V>(k, x);
+    float m = x[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float t = d.slow(x[v], s), e = exp2_fast(t);
-      p.s += e;
-      p.q = fmaf(e, t, p.q);
-    }
+    for (int v = 1; v < V; ++v) m = max_nan(m, x[v]);
+    return m;
   }
 }
+template <class T, int V> APPY_DEV void unpack_from(const Pack<T, V>& k, unsigned bound, float (&x)[V]) {
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    typename Pack<T, V>::Bits u;
+    u.raw = k.raw;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, bf16>::value) asm("max.bf16x2 %0, %0, %1;" : "+r"(u.w[i]) : "r"(bound));
+      else asm("max.f16x2 %0, %0, %1;" : "+r"(u.w[i]) : "r"(bound));
+      unpack2(u.w[i], x[2 * i], x[2 * i + 1], T());
+    }
+  } else {
+    unpack<T, V>(k, x);
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = fmaxf(x[v], sizeof(T) == 2 ? neg_inf() : __uint_as_float(bound));
+  }
+}
+// The bound for a maximum: so far below that the weight is zero, as two elements of T (or one float32).  False: none
+// that is finite in T, or the maximum is far out; d is then held up one by one.
+template <class T> APPY_DEV bool bound_of(const Scaled& d, const Scale& s, unsigned& bound) {
+  const float b = d.m - s.span;
+  if constexpr (sizeof(T) == 4) {
+    bound = __float_as_uint(b);
+  } else if constexpr (std::is_same<T, bf16>::value) {
+    const unsigned short h = __bfloat16_as_ushort(__float2bfloat16_rd(b));
+    bound = h | (unsigned)h << 16;
+  } else {
+    if (!(b > -65504.f)) return false;
+    const unsigned short h = __half_as_ushort(__float2half_rd(b));
+    bound = h | (unsigned)h << 16;
+  }
+  return fabsf(d.m) <= s.span * 65536.f && !d.far;             // else m - span may be m
+}
+
+// One thread's part of a row: softmax with its own maximum, S and Q as pairs of sums.
+template <class T> struct Running {
+  float m;
+  bool fine;                 // a finite bound: whole packs at a time
+  unsigned bound;
+  Vec<2> s, q;
+  APPY_DEV void start() {
+    m = neg_inf();
+    fine = false;
+    bound = 0;
+    s = q = all<2>(0.f);
+  }
+  APPY_DEV Part part() const {
+    float a[2], b[2];
+    floats<2>(s, a);
+    floats<2>(q, b);
+    return {m, a[0] + a[1], b[0] + b[1]};
+  }
+  APPY_DEV void raise(float to, const Scale& sc) {
+    const Part p = rescaled(part(), max_nan(to, m), sc);         // a NaN stays
+    m = p.m;
+    const float a[2] = {p.s, 0.f}, b[2] = {p.q, 0.f};
+    s = vec<2>(a);
+    q = vec<2>(b);
+    fine = bound_of<T>(Scaled(m, sc), sc, bound);
+  }
+  template <int V> APPY_DEV void add_pack(const Pack<T, V>& k, const Scaled& d, const Scale& sc) {
+    if (fine && V > 1) {
+      float x[V];
+      unpack_from<T, V>(k, bound, x);
+#pragma unroll
+      for (int v = 0; v < V; v += 2) {
+        const float pr[2] = {x[v], x[V > 1 ? v + 1 : v]};
+        const Vec<2> t = fma<2>(vec<2>(pr), all<2>(sc.k), all<2>(-d.mk));
+        float e[2];
+        floats<2>(t, e);
+        e[0] = exp2_fast(e[0]);
+        e[1] = exp2_fast(e[1]);
+        const Vec<2> w = vec<2>(e);
+        s = add<2>(s, w);
+        q = fma<2>(w, t, q);
+      }
+    } else if (fabsf(m) < __int_as_float(0x7f800000)) {
+      float x[V], es = 0.f, eq = 0.f;
+      unpack<T, V>(k, x);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float t = d.far ? d.slow(x[v], sc) : d.fast(x[v], sc), e = exp2_fast(t);
+        es += e;
+        eq = fmaf(e, t, eq);
+      }
+      const float a[2] = {es, 0.f}, b[2] = {eq, 0.f};
+      s = add<2>(s, vec<2>(a));
+      q = add<2>(q, vec<2>(b));
+    }
+  }
+  // U packs whose first elements are at `at`, `at + step`, ..
+  template <int V, int U, bool TOP> APPY_DEV void take(const Pack<T, V> (&k)[U], int at, int step, Best& best, const Scale& sc) {
+    float top = neg_inf();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float pm = pack_max<T, V>(k[u]);
+      if (TOP) {
+        const unsigned o = ordered(pm);
+        if (o > best.value) best = {o, at + u * step};
+      }
+      top = u ? max_nan(top, pm) : pm;
+    }
+    if (!(top <= m)) raise(top, sc);
+    const Scaled d(m, sc);
+#pragma unroll
+    for (int u = 0; u < U; ++u) add_pack<V>(k[u], d, sc);
+  }
+};
 
 struct LogprobArgs {
   const void* logits;
@@ -155,8 +259,9 @@ struct LargerKey {
   template <class K> static APPY_DEV K op(K a, K b) { return a > b ? a : b; }
 };
 struct NoTop {};
-struct TopState {
-  u64 key[kBlock];
+template <int NT> struct TopState {
+  static constexpr int kGroups = NT < 64 ? NT : 64, kCandidates = NT < 64 ? 512 : 1024;
+  u64 key[NT];
   u64 found[kCandidates];
   u64 list[kTopMax];
   u64 bound;
@@ -164,8 +269,9 @@ struct TopState {
 };
 
 // The `top` largest keys of this block's part of the row, largest first, in t.list (0: there are fewer).
-template <class T, int V> APPY_DEV void select_top(TopState& t, const Best& best, bool any, const T* row, const Split& sp, int lo, int hi,
+template <class T, int V, int NT> APPY_DEV void select_top(TopState<NT>& t, const Best& best, bool any, const T* row, const Split& sp, int lo, int hi,
                                                    bool edges, int cols, int top) {
+  constexpr int kBlock = NT, kGroups = TopState<NT>::kGroups, kCandidates = TopState<NT>::kCandidates;
   const int tid = threadIdx.x;
   t.key[tid] = any ? ((u64)best.value << 32) | (unsigned)~best.at : 0;
   if (tid < kTopMax) t.list[tid] = 0;
@@ -240,13 +346,13 @@ template <class T, int V> APPY_DEV void select_top(TopState& t, const Best& best
 }
 
 // One cluster of C blocks per row; block `rank` takes an equal share of the packs, block 0 the elements around them.
-template <class T, int V, int C, bool TOP>
-__global__ void __launch_bounds__(kBlock, 2) k_logprobs(LogprobArgs a) {
-  constexpr int U = 4;
+template <class T, int V, int NT, int C, bool TOP>
+__global__ void __launch_bounds__(NT, 1024 / NT > 16 ? 16 : 1024 / NT) k_logprobs(LogprobArgs a) {
+  constexpr int U = NT == 32 ? 2 : 4, kBlock = NT, kWarps = NT / 32;
   __shared__ Part warp_part[kWarps];
   __shared__ Part parts[C];
   __shared__ u64 lists[TOP ? C : 1][TOP ? kTopMax : 1];
-  __shared__ typename std::conditional<TOP, TopState, NoTop>::type top_state;
+  __shared__ typename std::conditional<TOP, TopState<NT>, NoTop>::type top_state;
   const int tid = threadIdx.x, rank = C > 1 ? blockIdx.x % C : 0;
   const i64 n = blockIdx.x / C;
   const T* const row = static_cast<const T*>(a.logits) + n * a.ld;
@@ -259,36 +365,40 @@ __global__ void __launch_bounds__(kBlock, 2) k_logprobs(LogprobArgs a) {
     token = a.wide ? __ldg(static_cast<const i64*>(a.tokens) + n) : (i64)__ldg(static_cast<const int*>(a.tokens) + n);
     if (token >= 0 && token < a.cols) token_logit = to_f32(row[token]);
   }
-  Part p = {neg_inf(), 0.f, 0.f};
+  Running<T> run;
+  run.start();
   Best best = {0, 0};
   bool any = false;
   auto single = [&](int at) {
-    float x[1] = {to_f32(row[at])};
-    take<1, TOP>(x, at, p, best, a.scale);
+    Pack<T, 1> k[1] = {ld_keep<T, 1>(row + at)};
+    run.template take<1, 1, TOP>(k, at, 0, best, a.scale);
     any = true;
   };
-  if (edges && tid < sp.head) single(tid);
-  for (int p0 = lo + tid; p0 < hi; p0 += kBlock * U) {
+  if (edges)
+    for (int at = tid; at < sp.head; at += kBlock) single(at);
+  const T* const body = row + sp.head;
+  int p0 = lo + tid;
+  for (; p0 + (U - 1) * kBlock < hi; p0 += kBlock * U) {
     Pack<T, V> k[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (p0 + u * kBlock < hi) k[u] = ld_stream<T, V>(row + sp.head + (p0 + u * kBlock) * V);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (p0 + u * kBlock < hi) {
-        float x[V];
-        unpack<T, V>(k[u], x);
-        take<V, TOP>(x, sp.head + (p0 + u * kBlock) * V, p, best, a.scale);
-      }
+    for (int u = 0; u < U; ++u) k[u] = ld_stream<T, V>(body + (i64)(p0 + u * kBlock) * V);
+    run.template take<V, U, TOP>(k, sp.head + p0 * V, kBlock * V, best, a.scale);
     any = true;
   }
-  if (edges && sp.tail0 + tid < a.cols) single(sp.tail0 + tid);
+  for (; p0 < hi; p0 += kBlock) {
+    Pack<T, V> k[1] = {ld_stream<T, V>(body + (i64)p0 * V)};
+    run.template take<V, 1, TOP>(k, sp.head + p0 * V, 0, best, a.scale);
+    any = true;
+  }
+  if (edges)
+    for (int at = sp.tail0 + tid; at < a.cols; at += kBlock) single(at);
+  Part p = run.part();
   for (int o = 16; o; o >>= 1) {
     const Part y = {__shfl_xor_sync(APPY_FULL_MASK, p.m, o), __shfl_xor_sync(APPY_FULL_MASK, p.s, o), __shfl_xor_sync(APPY_FULL_MASK, p.q, o)};
     p = joined(p, y, a.scale);
   }
   if ((tid & 31) == 0) warp_part[tid >> 5] = p;
-  if constexpr (TOP) select_top<T, V>(top_state, best, any, row, sp, lo, hi, edges, a.cols, a.top);
+  if constexpr (TOP) select_top<T, V, NT>(top_state, best, any, row, sp, lo, hi, edges, a.cols, a.top);
   __syncthreads();
   if (tid == 0) {
     p = warp_part[0];
@@ -307,11 +417,12 @@ __global__ void __launch_bounds__(kBlock, 2) k_logprobs(LogprobArgs a) {
       for (int r = 1; r < C; ++r) p = joined(p, parts[r], a.scale);
     }
     if constexpr (TOP) {
-      for (int x = tid; x < C * kTopMax; x += kBlock) {
-        const u64 k = lists[x / kTopMax][x % kTopMax];
+      for (int x = tid; x < C * a.top; x += kBlock) {
+        const u64 k = lists[x / a.top][x % a.top];
         if (!k) continue;
         int above = 0;
-        for (int y = 0; y < C * kTopMax; ++y) above += lists[y / kTopMax][y % kTopMax] > k;
+        for (int r = 0; r < C; ++r)
+          for (int y = 0; y < a.top; ++y) above += lists[r][y] > k;
         if (above < a.top) top_state.list[above] = k;
       }
     }
@@ -379,6 +490,8 @@ __global__ void __launch_bounds__(kGradBlock) k_logprobs_grad(LogprobGradArgs a)
   // d logits = p * (c0 + c1 * log2 p) + [j = token] * c2
   const float c0 = -(g + gh * h) * a.scale.inv_temperature, c1 = -gh * kLn2 * a.scale.inv_temperature, c2 = empty ? 0.f : g * a.scale.inv_temperature;
   const Scaled d(m, a.scale);
+  unsigned bound;
+  const bool fine = bound_of<T>(d, a.scale, bound) && !empty && !bad && V > 1;
   auto one = [&](float x, int at) {
     const float t = (d.far ? d.slow(x, a.scale) : d.fast(x, a.scale)) - log2s;
     float r = exp2_fast(t) * fmaf(c1, t, c0);
@@ -390,15 +503,30 @@ __global__ void __launch_bounds__(kGradBlock) k_logprobs_grad(LogprobGradArgs a)
   Pack<T, V> k[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (p0 + u * kGradBlock < sp.packs) k[u] = ld_stream<T, V>(row + sp.head + (p0 + u * kGradBlock) * V);
+    if (p0 + u * kGradBlock < sp.packs) k[u] = ld_stream<T, V>(row + sp.head + (i64)(p0 + u * kGradBlock) * V);
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (p0 + u * kGradBlock < sp.packs) {
       const int at = sp.head + (p0 + u * kGradBlock) * V;
       float x[V];
-      unpack<T, V>(k[u], x);
+      if (fine) {
+        unpack_from<T, V>(k[u], bound, x);
+        const Vec<V> t = add<V>(fma<V>(vec<V>(x), all<V>(a.scale.k), all<V>(-d.mk)), all<V>(-log2s));
+        float e[V];
+        floats<V>(t, e);
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = one(x[v], at + v);
+        for (int v = 0; v < V; ++v) e[v] = exp2_fast(e[v]);
+        floats<V>(mul<V>(vec<V>(e), fma<V>(t, all<V>(c1), all<V>(c0))), x);
+        if ((unsigned)((int)token - at) < (unsigned)V) {
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (at + v == (int)token) x[v] += c2;
+        }
+      } else {
+        unpack<T, V>(k[u], x);
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = one(x[v], at + v);
+      }
       st_stream<T, V>(out + at, pack<T, V>(x));
     }
   if (V > 1 && chunk == 0) {
@@ -409,10 +537,10 @@ __global__ void __launch_bounds__(kGradBlock) k_logprobs_grad(LogprobGradArgs a)
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <class T, int V, int C, bool TOP> int launch_c(const LogprobArgs& a, i64 rows, cudaStream_t s) {
+template <class T, int V, int NT, int C, bool TOP> int launch_c(const LogprobArgs& a, i64 rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * C));
-  cfg.blockDim = dim3(kBlock);
+  cfg.blockDim = dim3(NT);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -420,7 +548,7 @@ template <class T, int V, int C, bool TOP> int launch_c(const LogprobArgs& a, i6
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_logprobs<T, V, C, TOP>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_logprobs<T, V, NT, C, TOP>, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return appy_fail_cuda(e, "token logprobs launch");
@@ -430,20 +558,24 @@ template <class T, int V, int C, bool TOP> int launch_c(const LogprobArgs& a, i6
 
 template <class T, bool TOP> int launch_logprobs(const LogprobArgs& a, i64 rows, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  // few rows: a cluster of up to 8 blocks per row, as long as every thread still has a pack
+  // a block per row, of so many threads that each has some packs: short rows would otherwise wait at barriers for
+  // threads without work.  Few long rows: a cluster of up to 8 blocks per row, as long as every thread still has two.
+  const i64 packs = a.cols / V, sms = sm_count();
+  if (packs <= 256) return launch_c<T, V, 32, 1, TOP>(a, rows, s);
+  if (packs <= 2048 && rows >= sms) return launch_c<T, V, 128, 1, TOP>(a, rows, s);
   int c = 1;
-  while (c < 8 && rows * c < 2 * (i64)sm_count() && a.cols / V >= kBlock * 2 * c) c *= 2;
+  while (c < 8 && rows * c < 2 * sms && packs >= 512 * 2 * c) c *= 2;
   switch (c) {
-    case 1: return launch_c<T, V, 1, TOP>(a, rows, s);
-    case 2: return launch_c<T, V, 2, TOP>(a, rows, s);
-    case 4: return launch_c<T, V, 4, TOP>(a, rows, s);
-    default: return launch_c<T, V, 8, TOP>(a, rows, s);
+    case 1: return launch_c<T, V, 512, 1, TOP>(a, rows, s);
+    case 2: return launch_c<T, V, 512, 2, TOP>(a, rows, s);
+    case 4: return launch_c<T, V, 512, 4, TOP>(a, rows, s);
+    default: return launch_c<T, V, 512, 8, TOP>(a, rows, s);
   }
 }
 
 Scale scale_of(float temperature) {
   const float k = 1.44269504088896341f / temperature;
-  return {k, 1e38f / (k > 1.f ? k : 1.f), 1.f / temperature};
+  return {k, 1e38f / (k > 1.f ? k : 1.f), 200.f / k, 1.f / temperature};
 }
 
 int check_logits(const char* fn, int dtype, int token_dtype, i64 rows, i64 cols, i64 ld, float temperature) {

@@ -122,6 +122,57 @@ template <class T, int V> APPY_DEV Pack<T, V> pack(const float (&f)[V]) {
   return {u.raw};
 }
 
+// ------------------------------------------------------------------------------------------------ V floats at a time
+// Two float32 of one 64-bit register per instruction where V is even: kernels that issue a dozen operations per element
+// are bound by that, and products and sums of pairs cost half.
+template <int V> struct Vec { u64 p[V / 2]; };
+template <> struct Vec<1> { float p[1]; };
+
+APPY_DEV u64 pair(float lo, float hi) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+APPY_DEV float mul1(float a, float b) { return a * b; }
+APPY_DEV float add1(float a, float b) { return a + b; }
+APPY_DEV u64 mul1(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+APPY_DEV u64 add1(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+APPY_DEV float fma1(float a, float b, float c) { return fmaf(a, b, c); }
+APPY_DEV u64 fma1(u64 a, u64 b, u64 c) { u64 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+template <int V> APPY_DEV Vec<V> vec(const float (&f)[V]) {
+  Vec<V> r;
+  if constexpr (V == 1) {
+    r.p[0] = f[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = pair(f[2 * i], f[2 * i + 1]);
+  }
+  return r;
+}
+template <int V> APPY_DEV Vec<V> all(float x) {
+  float f[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = x;
+  return vec<V>(f);
+}
+template <int V> APPY_DEV void floats(const Vec<V>& a, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = a.p[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) asm("mov.b64 {%0, %1}, %2;" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "l"(a.p[i]));
+  }
+}
+#define APPY_EACH(expr)                                                    \
+  Vec<V> r;                                                                \
+  _Pragma("unroll") for (int i = 0; i < (V == 1 ? 1 : V / 2); ++i) r.p[i] = expr; \
+  return r
+template <int V> APPY_DEV Vec<V> mul(const Vec<V>& a, const Vec<V>& b) { APPY_EACH(mul1(a.p[i], b.p[i])); }
+template <int V> APPY_DEV Vec<V> add(const Vec<V>& a, const Vec<V>& b) { APPY_EACH(add1(a.p[i], b.p[i])); }
+template <int V> APPY_DEV Vec<V> fma(const Vec<V>& a, const Vec<V>& b, const Vec<V>& c) { APPY_EACH(fma1(a.p[i], b.p[i], c.p[i])); }
+#undef APPY_EACH
+
 // ------------------------------------------------------------------------------------------------ host side
 inline int sm_count() {
   static int known[16] = {0};
