@@ -297,16 +297,21 @@ template <class T, int V, int NT> APPY_DEV void select_top(TopState<NT>& t, cons
     const int n = atomicAdd(&t.count, 1);
     if (n < kCandidates) t.found[n] = key_of(v, at);
   };
-  if (any && own >= bound) {
-    if (edges && tid < sp.head) look(to_f32(row[tid]), tid, tid);
-    for (int p = lo + tid; p < hi; p += kBlock) {
+  const bool again = any && own >= bound;
+  if (again && edges) {
+    if (tid < sp.head) look(to_f32(row[tid]), tid, tid);
+    if (sp.tail0 + tid < cols) look(to_f32(row[sp.tail0 + tid]), sp.tail0 + tid, sp.tail0 + tid);
+  }
+  // the packs of a thread that has candidates are looked through by its whole warp
+  for (unsigned who = __ballot_sync(APPY_FULL_MASK, again); who; who &= who - 1) {
+    const int other = (tid & ~31) + __ffs(who) - 1;
+    for (int p = lo + other + (tid & 31) * kBlock; p < hi; p += 32 * kBlock) {
       const int at = sp.head + p * V;
       float x[V];
       unpack<T, V>(ld_keep<T, V>(row + at), x);
 #pragma unroll
       for (int v = 0; v < V; ++v) look(x[v], at, at + v);
     }
-    if (edges && sp.tail0 + tid < cols) look(to_f32(row[sp.tail0 + tid]), sp.tail0 + tid, sp.tail0 + tid);
   }
   __syncthreads();
   const int count = t.count;
@@ -420,9 +425,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT > 16 ? 16 : 1024 / NT) k_logprob
       for (int x = tid; x < C * a.top; x += kBlock) {
         const u64 k = lists[x / a.top][x % a.top];
         if (!k) continue;
-        int above = 0;
-        for (int r = 0; r < C; ++r)
-          for (int y = 0; y < a.top; ++y) above += lists[r][y] > k;
+        int above = 0;                                   // keys above this one in each block's list, which falls
+#pragma unroll
+        for (int r = 0; r < C; ++r) {
+          int n = 0;
+#pragma unroll
+          for (int step = 32; step; step >>= 1)
+            if (n + step <= a.top && lists[r][n + step - 1] > k) n += step;
+          above += n;
+        }
         if (above < a.top) top_state.list[above] = k;
       }
     }
@@ -561,12 +572,12 @@ template <class T, bool TOP> int launch_logprobs(const LogprobArgs& a, i64 rows,
   // a block per row, of so many threads that each has some packs: short rows would otherwise wait at barriers for
   // threads without work.  Few long rows: a cluster of up to 8 blocks per row, as long as every thread still has two.
   const i64 packs = a.cols / V, sms = sm_count();
-  if (packs <= 256) return launch_c<T, V, 32, 1, TOP>(a, rows, s);
+  if (packs <= (rows >= 8 * sms ? 1024 : 256)) return launch_c<T, V, 32, 1, TOP>(a, rows, s);
   if (packs <= 2048 && rows >= sms) return launch_c<T, V, 128, 1, TOP>(a, rows, s);
   int c = 1;
   while (c < 8 && rows * c < 2 * sms && packs >= 512 * 2 * c) c *= 2;
   switch (c) {
-    case 1: return launch_c<T, V, 512, 1, TOP>(a, rows, s);
+    case 1: return launch_c<T, V, 256, 1, TOP>(a, rows, s);
     case 2: return launch_c<T, V, 512, 2, TOP>(a, rows, s);
     case 4: return launch_c<T, V, 512, 4, TOP>(a, rows, s);
     default: return launch_c<T, V, 512, 8, TOP>(a, rows, s);
