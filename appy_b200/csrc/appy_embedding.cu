@@ -68,6 +68,39 @@ __global__ void __launch_bounds__(kLookupBlock) k_lookup(const T* __restrict__ w
   }
 }
 
+// Rows that packs cannot move: a warp takes kLookupCols neighbouring elements of a row, so that no element needs an
+// index of its own (30000 rows of 1001 bfloat16: the flat form with single elements 91 us).
+const int kLookupCols = 512;
+
+template <class T>
+__global__ void __launch_bounds__(kLookupBlock) k_lookup_single(const T* __restrict__ w, i64 ldw, i64 rows, i64 width, int parts,
+                                                                const void* __restrict__ tokens, bool wide, i64 n, float scale,
+                                                                T* __restrict__ out, i64 ldo) {
+  constexpr int U = 8;
+  const int lane = threadIdx.x & 31;
+  const i64 unit = (i64)blockIdx.x * (kLookupBlock / 32) + (threadIdx.x >> 5), row = unit / parts;
+  if (row >= n) return;
+  const i64 lo = (unit - row * parts) * kLookupCols, hi = min(lo + kLookupCols, width), tok = token_of(tokens, wide, row);
+  const bool known = tok >= 0 && tok < rows;
+  const T* const from = w + (known ? tok * ldw : 0);
+  T* const to = out + row * ldo;
+  for (i64 c = lo + lane; c < hi; c += 32 * U) {
+    Pack<T, 1> k[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k[u] = zero_pack<T, 1>();
+      if (known && c + 32 * u < hi) k[u] = ld_keep<T, 1>(from + c + 32 * u);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[1];
+      unpack<T, 1>(k[u], f);
+      f[0] *= scale;
+      if (c + 32 * u < hi) st_stream<T, 1>(to + c + 32 * u, scale == 1.f ? k[u] : pack<T, 1>(f));
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ sort by token
 // Stable radix sort of (key, position), least significant digit first.  The key of a position is its token, or
 // `rows` for one that is dropped, so dropped positions come last.  A block owns a contiguous range of positions;
@@ -729,15 +762,16 @@ int appy_embedding(const void* dweight, int dtype, int64_t ldw, int64_t rows, in
   const bool wide = token_dtype == APPY_I64;
   const int V = 16 / size;
   const bool vec = width % V == 0 && ldw % V == 0 && ldo % V == 0 && aligned(dweight, 16) && aligned(dout, 16);
-  const i64 per_row = vec ? width / V : width, total = n * per_row, blocks = (total + kLookupBlock * 4 - 1) / (kLookupBlock * 4);
+  const i64 parts = (width + kLookupCols - 1) / kLookupCols, warps = kLookupBlock / 32;
+  const i64 blocks = vec ? (n * (width / V) + kLookupBlock * 4 - 1) / (kLookupBlock * 4) : (n * parts + warps - 1) / warps;
   if (blocks > 0x7fffffff) return fail_named(fn, "too many elements for one launch");
   return APPY_OP_DTYPE(dtype, {
     const T* w = static_cast<const T*>(dweight);
     T* out = static_cast<T*>(dout);
     if (vec)
-      k_lookup<T, 16 / sizeof(T), 4><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, (unsigned)per_row, dtokens, wide, n, scale, out, ldo);
+      k_lookup<T, 16 / sizeof(T), 4><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, (unsigned)(width / V), dtokens, wide, n, scale, out, ldo);
     else
-      k_lookup<T, 1, 4><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, (unsigned)per_row, dtokens, wide, n, scale, out, ldo);
+      k_lookup_single<T><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, width, (int)parts, dtokens, wide, n, scale, out, ldo);
     return finish("embedding launch");
   });
 }

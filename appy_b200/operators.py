@@ -160,13 +160,29 @@ def _like(fn, name, t, shape, dtype):
         _fail(fn, f"{name} must be {dtype} of shape {tuple(shape)}, got {t.dtype} of {tuple(t.shape)}")
 
 
+_entries: dict = {}
+_one_device = None
+
+
+def _entry(name):
+    """The C function `name`; the library's own set-up of the device comes with the first."""
+    global _one_device
+    if _one_device is None:
+        _one_device = torch.cuda.device_count() == 1
+        rt.init(torch.cuda.current_device())
+    fn = _entries[name] = getattr(rt.lib(), name)
+    return fn
+
+
 def _run(entry, device, *args):
     """Call the C entry on torch's current stream of `device`."""
-    if torch.cuda.current_device() != device:
+    if torch._C._cuda_getDevice() != device:
         with torch.cuda.device(device):
             return _run(entry, device, *args)
-    lib = rt._LIB or rt.lib()
-    if lib.appy_init(device) or getattr(lib, entry)(*args, torch._C._cuda_getCurrentRawStream(device)):
+    fn = _entries.get(entry) or _entry(entry)
+    if not _one_device:
+        rt.init(device)                            # with several, the library's idea of the current one follows torch's
+    if fn(*args, torch._C._cuda_getCurrentRawStream(device)):
         rt.check(-1)
 
 
@@ -404,15 +420,19 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     device = _together(fn, logits, tokens)
     logits, ld = _rows_in(logits)
     tokens = tokens.contiguous()
-    shape = tokens.shape
-    dev = logits.device
-    logprobs, entropy = torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev)
-    stats = torch.empty(shape + (3,), dtype=torch.float32, device=dev)
-    top_logprobs = top_tokens = None
+    shape, n, dev = tokens.shape, tokens.numel(), logits.device
+    # one allocation for the float32 results: an allocation costs the host more than a view
+    logprobs, entropy, stats, top_logprobs = torch.empty(n * (5 + top), dtype=torch.float32, device=dev).split((n, n, 3 * n, top * n))
+    stats = stats.view(shape + (3,))
+    if len(shape) != 1:
+        logprobs, entropy = logprobs.view(shape), entropy.view(shape)
+    top_tokens = None
     if top:
-        top_logprobs = torch.empty(shape + (top,), dtype=torch.float32, device=dev)
+        top_logprobs = top_logprobs.view(shape + (top,))
         top_tokens = torch.empty(shape + (top,), dtype=tokens.dtype, device=dev)
-    _run("appy_token_logprobs", device, logits.data_ptr(), code, ld, tokens.numel(), cols, tokens.data_ptr(), int_code, temperature, top,
+    else:
+        top_logprobs = None
+    _run("appy_token_logprobs", device, logits.data_ptr(), code, ld, n, cols, tokens.data_ptr(), int_code, temperature, top,
          logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr(), _ptr(top_logprobs), _ptr(top_tokens))
     return LogProbs(logprobs, entropy, stats, top_logprobs, top_tokens)
 
