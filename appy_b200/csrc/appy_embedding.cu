@@ -800,6 +800,7 @@ int appy_embedding_grad(const void* dgrad, int dtype, int64_t ldg, const void* d
   const int V = grad_vec(dgrad, dtype, ldg, dout, out_dtype, ldo, width);
   const GradPlan p = grad_plan(n, rows, width, V);
   if (n && (workspace_bytes < p.bytes || !aligned(dworkspace, 256))) return fail_named(fn, "workspace too small or not aligned to 256 bytes");
+  if (n <= kFewTokens && n * p.col_warps > 0x7fffffff) return fail_named(fn, "too many elements for one launch");
   if (n && n <= kFewTokens) {
     const int blocks = (int)((n * p.col_warps + 7) / 8);
     const FewArgs a{dtokens, token_dtype == APPY_I64, (int)n, (int)rows, p.col_warps, blocks, width, ldg, ldo, scale, accumulate != 0,

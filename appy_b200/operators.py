@@ -12,7 +12,9 @@ in place, such as a transposed last dimension, is copied first); arrays that are
 
 Gradients are functions of their own: nothing is recorded for autograd, and a tensor that requires grad is refused
 while grad mode is on.  A ``torch.autograd.Function`` whose ``forward`` calls ``f`` and whose ``backward`` calls
-``f_grad`` puts an operator into a graph.  Calls may be captured into CUDA graphs, gradients included.
+``f_grad`` puts an operator into a graph.  Calls may be captured into CUDA graphs, gradients included, once each kind of
+call has run outside of one (kernels are loaded with their first call).  An array that is written must not overlap an
+argument, unless it says so.
 """
 from __future__ import annotations
 
@@ -208,8 +210,8 @@ def embedding(weight, tokens, scale=1.0, out=None):
         out, ldo = torch.empty(shape, dtype=weight.dtype, device=weight.device), width
     else:
         ldo = _rows_out(fn, "out", out, shape, weight.dtype)
-    _run("appy_embedding", device, weight.data_ptr(), code, ldw, rows, width, tokens.data_ptr(), int_code, tokens.numel(), scale,
-         out.data_ptr(), ldo)
+    _run("appy_embedding", device, weight.data_ptr(), code, ldw, rows, width, tokens.data_ptr(), int_code, tokens.numel(),
+         float(scale), out.data_ptr(), ldo)
     return out
 
 
@@ -257,7 +259,7 @@ def embedding_grad(grad, tokens, rows=None, scale=1.0, out=None, accumulate=Fals
     tokens = tokens.contiguous()
     n = tokens.numel()
     workspace = torch.empty(_embedding_grad_bytes(n, rows, width), dtype=torch.uint8, device=grad.device)
-    _run("appy_embedding_grad", device, grad.data_ptr(), code, ldg, tokens.data_ptr(), int_code, n, rows, width, scale, bool(accumulate),
+    _run("appy_embedding_grad", device, grad.data_ptr(), code, ldg, tokens.data_ptr(), int_code, n, rows, width, float(scale), bool(accumulate),
          out.data_ptr(), _FLOATS[out.dtype], ldo, workspace.data_ptr(), workspace.numel())
     return out
 
@@ -432,7 +434,7 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
         top_tokens = torch.empty(shape + (top,), dtype=tokens.dtype, device=dev)
     else:
         top_logprobs = None
-    _run("appy_token_logprobs", device, logits.data_ptr(), code, ld, n, cols, tokens.data_ptr(), int_code, temperature, top,
+    _run("appy_token_logprobs", device, logits.data_ptr(), code, ld, n, cols, tokens.data_ptr(), int_code, float(temperature), top,
          logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr(), _ptr(top_logprobs), _ptr(top_tokens))
     return LogProbs(logprobs, entropy, stats, top_logprobs, top_tokens)
 
@@ -471,5 +473,5 @@ def token_logprobs_grad(logits, tokens, stats, grad_logprobs=None, grad_entropy=
     logits, ld = _rows_in(logits)
     tokens, stats = tokens.contiguous(), stats.contiguous()
     _run("appy_token_logprobs_grad", device, logits.data_ptr(), code, ld, tokens.numel(), logits.shape[-1], tokens.data_ptr(), int_code,
-         temperature, stats.data_ptr(), _ptr(g), g_stride, _ptr(gh), gh_stride, out.data_ptr(), ldo)
+         float(temperature), stats.data_ptr(), _ptr(g), g_stride, _ptr(gh), gh_stride, out.data_ptr(), ldo)
     return out

@@ -567,6 +567,46 @@ def test_token_logprobs_gradient_against_differences(rt):
         assert abs(float(loss(up) - loss(down)) / 2e-6 - float(got.view(-1)[k])) < 1e-4
 
 
+# ------------------------------------------------------------------------------------------------ large arrays
+
+def test_offsets_past_32_bits(rt):
+    """Arrays of more than 2^31 elements: their last rows agree with calls on those rows alone."""
+    rows, width = (1 << 19) + 5, 4104                                     # 2.15e9 elements
+    w = torch.empty(rows, width, dtype=torch.bfloat16, device="cuda")
+    w[-64:] = randn(64, width, dtype=torch.bfloat16, seed=1)
+    w[:64] = 1.0
+    tokens = torch.randint(rows - 64, rows, (50,), generator=gen(2), device="cuda")
+    assert torch.equal(appy.embedding(w, tokens), w[tokens])
+    grad = randn(50, width, dtype=torch.bfloat16, seed=3)
+    appy.embedding_grad(grad, tokens, out=w)
+    assert torch.equal(w[-64:], appy.embedding_grad(grad, tokens - (rows - 64), 64)) and not w[:64].any() and not w[rows // 2].any()
+    tokens = torch.randint(rows - 64, rows, (5000,), generator=gen(4), device="cuda")
+    grad = randn(5000, width, dtype=torch.bfloat16, seed=5)
+    appy.embedding_grad(grad, tokens, out=w)
+    assert torch.equal(w[-64:], appy.embedding_grad(grad, tokens - (rows - 64), 64)) and not w[:64].any()
+    del w
+    n, cols = 16400, 131072
+    logits = torch.zeros(n, cols, dtype=torch.bfloat16, device="cuda")
+    logits[-8:] = randn(8, cols, dtype=torch.bfloat16, seed=6)
+    tokens = torch.randint(0, cols, (n,), generator=gen(7), device="cuda")
+    g = randn(n, seed=8)
+    r = appy.token_logprobs(logits, tokens, top=3)
+    few = appy.token_logprobs(logits[-8:], tokens[-8:], top=3)
+    within(r.logprobs[-8:], few.logprobs.double(), logprob_tolerance(cols) + 8 * U * few.logprobs.double().abs())
+    assert torch.equal(r.top_tokens[-8:], few.top_tokens)
+    want = appy.token_logprobs_grad(logits[-8:], tokens[-8:], r.stats[-8:], g[-8:])
+    appy.token_logprobs_grad(logits, tokens, r.stats, g, out=logits)
+    assert torch.equal(logits[-8:], want)
+    del logits
+    t, d = (1 << 20) + 3, 2056
+    x = torch.zeros(1, t, d, dtype=torch.bfloat16, device="cuda")
+    x[:, -300:] = randn(1, 300, d, dtype=torch.bfloat16, seed=9)
+    h, last = appy.gated_scan(x, x)
+    end, last2 = appy.gated_scan(x[:, -300:], x[:, -300:])
+    within(last, last2.double(), 1e-5 + 1e-5 * last2.double().abs())
+    within(h[:, -300:], end.double(), 2 * half(torch.bfloat16) * end.double().abs() + 1e-5)
+
+
 # ------------------------------------------------------------------------------------------------ as they are used
 
 def test_refusals(rt):
