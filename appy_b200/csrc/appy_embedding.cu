@@ -27,8 +27,10 @@ APPY_DEV i64 token_of(const void* tokens, bool wide, i64 n) {
 }
 
 // ------------------------------------------------------------------------------------------------ lookup
-// Flat over the packs of the output: pack i belongs to row i / per_row.  A thread has U packs a block apart in
-// flight (token, then row); neighbouring threads read one row, so token loads are broadcasts.
+// Rows of at least 32 packs: a warp takes a stretch of one row, so that no pack needs an index of its own (65536 rows
+// of 4096 bfloat16: the flat form issued 118 instructions per 32 packs, four fifths of all issue slots).  Shorter
+// rows: flat over the packs of the output, pack i of row i / per_row; neighbouring threads read one row, so token
+// loads are broadcasts.
 const int kLookupBlock = 256;
 
 template <class T, int V, int U>
@@ -68,36 +70,38 @@ __global__ void __launch_bounds__(kLookupBlock) k_lookup(const T* __restrict__ w
   }
 }
 
-// Rows that packs cannot move: a warp takes kLookupCols neighbouring elements of a row, so that no element needs an
-// index of its own (30000 rows of 1001 bfloat16: the flat form with single elements 91 us).
-const int kLookupCols = 512;
-
-template <class T>
-__global__ void __launch_bounds__(kLookupBlock) k_lookup_single(const T* __restrict__ w, i64 ldw, i64 rows, i64 width, int parts,
-                                                                const void* __restrict__ tokens, bool wide, i64 n, float scale,
-                                                                T* __restrict__ out, i64 ldo) {
-  constexpr int U = 8;
+// A warp takes `stretch` neighbouring packs of a row (elements, where packs cannot move it), U of them in flight a lane.
+template <class T, int V, int U>
+__global__ void __launch_bounds__(kLookupBlock) k_lookup_rows(const T* __restrict__ w, i64 ldw, i64 rows, i64 per_row, int parts, int stretch,
+                                                              const void* __restrict__ tokens, bool wide, i64 n, float scale,
+                                                              T* __restrict__ out, i64 ldo) {
   const int lane = threadIdx.x & 31;
   const i64 unit = (i64)blockIdx.x * (kLookupBlock / 32) + (threadIdx.x >> 5), row = unit / parts;
   if (row >= n) return;
-  const i64 lo = (unit - row * parts) * kLookupCols, hi = min(lo + kLookupCols, width), tok = token_of(tokens, wide, row);
+  const i64 lo = (unit - row * parts) * stretch, tok = token_of(tokens, wide, row);
+  const int count = (int)min((i64)stretch, per_row - lo);
   const bool known = tok >= 0 && tok < rows;
-  const T* const from = w + (known ? tok * ldw : 0);
-  T* const to = out + row * ldo;
-  for (i64 c = lo + lane; c < hi; c += 32 * U) {
-    Pack<T, 1> k[U];
+  const T* const from = w + (known ? tok * ldw : 0) + lo * V;
+  T* const to = out + row * ldo + lo * V;
+  for (int c = lane; c < count; c += 32 * U) {
+    Pack<T, V> k[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      k[u] = zero_pack<T, 1>();
-      if (known && c + 32 * u < hi) k[u] = ld_keep<T, 1>(from + c + 32 * u);
+      k[u] = zero_pack<T, V>();
+      if (known && c + 32 * u < count) k[u] = ld_keep<T, V>(from + (c + 32 * u) * V);
+    }
+    if (scale != 1.f) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f[V];
+        unpack<T, V>(k[u], f);
+        floats<V>(mul<V>(vec<V>(f), all<V>(scale)), f);
+        k[u] = pack<T, V>(f);
+      }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[1];
-      unpack<T, 1>(k[u], f);
-      f[0] *= scale;
-      if (c + 32 * u < hi) st_stream<T, 1>(to + c + 32 * u, scale == 1.f ? k[u] : pack<T, 1>(f));
-    }
+    for (int u = 0; u < U; ++u)
+      if (c + 32 * u < count) st_stream<T, V>(to + (c + 32 * u) * V, k[u]);
   }
 }
 
@@ -762,16 +766,20 @@ int appy_embedding(const void* dweight, int dtype, int64_t ldw, int64_t rows, in
   const bool wide = token_dtype == APPY_I64;
   const int V = 16 / size;
   const bool vec = width % V == 0 && ldw % V == 0 && ldo % V == 0 && aligned(dweight, 16) && aligned(dout, 16);
-  const i64 parts = (width + kLookupCols - 1) / kLookupCols, warps = kLookupBlock / 32;
-  const i64 blocks = vec ? (n * (width / V) + kLookupBlock * 4 - 1) / (kLookupBlock * 4) : (n * parts + warps - 1) / warps;
+  const i64 per_row = vec ? width / V : width, stretch = vec ? 128 : 512, parts = (per_row + stretch - 1) / stretch;
+  const bool flat = vec && per_row < 32;
+  const i64 blocks = flat ? (n * per_row + kLookupBlock * 4 - 1) / (kLookupBlock * 4) : (n * parts + kLookupBlock / 32 - 1) / (kLookupBlock / 32);
   if (blocks > 0x7fffffff) return fail_named(fn, "too many elements for one launch");
   return APPY_OP_DTYPE(dtype, {
+    constexpr int W = 16 / sizeof(T);
     const T* w = static_cast<const T*>(dweight);
     T* out = static_cast<T*>(dout);
-    if (vec)
-      k_lookup<T, 16 / sizeof(T), 4><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, (unsigned)(width / V), dtokens, wide, n, scale, out, ldo);
+    if (flat)
+      k_lookup<T, W, 4><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, (unsigned)per_row, dtokens, wide, n, scale, out, ldo);
+    else if (vec)
+      k_lookup_rows<T, W, 4><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, per_row, (int)parts, (int)stretch, dtokens, wide, n, scale, out, ldo);
     else
-      k_lookup_single<T><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, width, (int)parts, dtokens, wide, n, scale, out, ldo);
+      k_lookup_rows<T, 1, 8><<<(unsigned)blocks, kLookupBlock, 0, s>>>(w, ldw, rows, per_row, (int)parts, (int)stretch, dtokens, wide, n, scale, out, ldo);
     return finish("embedding launch");
   });
 }
