@@ -576,7 +576,8 @@ template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, 
 
 // Variants, each with the time of the one it was chosen over (B200, bfloat16 unless said, forward / gradient):
 //   many (sequence, 64 channels) pairs, four per SM: 64-channel blocks of 4 tokens per thread, four to an SM
-//     (64 x 512 x 2048: 71 us; 32-channel blocks of 8 tokens per thread 96 us);
+//     (64 x 512 x 2048: 71 us; 32-channel blocks of 8 tokens per thread 96 us), and short sequences (16 x 100 x 2048:
+//     8 / 12 us; the others 12 / 14 us);
 //   fewer: 32-channel blocks, twice as many; forward 8 tokens per thread and two blocks to an SM (8 x 2048 x 2048:
 //     46 us; the first variant 53 us), gradient 4 tokens per thread and four blocks (73 us; the first variant 94 us);
 //   fewer than two 32-channel blocks per SM: clusters along the tokens, as many blocks as keep to two per SM, which
@@ -587,7 +588,7 @@ template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t 
   constexpr bool wide = sizeof(T) == 4;
   constexpr int S = wide || BACK ? 2 : 4, LT = BACK ? 4 : 8;
   const i64 sms = sm_count(), units = a.sequences * ((a.width + 31) / 32), wide_units = a.sequences * ((a.width + 63) / 64);
-  if (wide_units >= 4 * sms || a.tokens <= 32) return launch_c<T, 4, 16, 4, S, 128, 1, BACK && wide ? 3 : 4, BACK>(a, s);
+  if (wide_units >= 4 * sms || a.tokens <= 128) return launch_c<T, 4, 16, 4, S, 128, 1, BACK && wide ? 3 : 4, BACK>(a, s);
   const i64 most = a.offsets ? 12 * sms : 2 * sms;
   int c = 1;
   while (c < 16 && units * 2 * c <= most && (i64)16 * LT * c < a.tokens) c *= 2;
@@ -599,7 +600,8 @@ template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t 
     default: return launch_c<T, 4, 8, LT, S, 128, 16, 2, BACK>(a, s);
   }
 }
-// Rows that TMA cannot read: the same with direct loads.
+// Rows that TMA cannot read: the same with direct loads (8 x 2048 x 1001 bfloat16 43 / 100 us; two channels a thread, for
+// packed arithmetic, 72 / 177 us: the loads are what takes the time).
 template <class T, bool BACK> int launch_direct(const ScanArgs& a, cudaStream_t s) {
   constexpr int LT = BACK ? 4 : 8;
   const i64 sms = sm_count(), units = a.sequences * ((a.width + 31) / 32);

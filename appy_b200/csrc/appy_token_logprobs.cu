@@ -569,11 +569,15 @@ template <class T, int V, int NT, int C, bool TOP> int launch_c(const LogprobArg
 
 template <class T, bool TOP> int launch_logprobs(const LogprobArgs& a, i64 rows, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  // a block per row, of so many threads that each has some packs: short rows would otherwise wait at barriers for
+  // A block per row, of so many threads that each has some packs: short rows would otherwise wait at barriers for
   // threads without work.  Few long rows: a cluster of up to 8 blocks per row, as long as every thread still has two.
+  // B200, bfloat16, 20 alternatives, microseconds for blocks of 32 / 128 / 256 threads:
+  //   8192 x 1000: 47 / 68 / 111,  8192 x 8192: 80 / 99 / 127,  8 x 1000: 14 / 8 / 10,  1000 x 8192: 25 / 17 / 21,
+  //   4000 x 16384: 73 / 68 / 84,  1000 x 32768: 96 / 31 / 35;  none, 4096 x 131072: 256 threads 198, 512 threads 226;
+  //   8 x 131072: clusters of 8 blocks 12.4, of 16 blocks 20.5.
   const i64 packs = a.cols / V, sms = sm_count();
-  if (packs <= (rows >= 8 * sms ? 1024 : 256)) return launch_c<T, V, 32, 1, TOP>(a, rows, s);
-  if (packs <= 2048 && rows >= sms) return launch_c<T, V, 128, 1, TOP>(a, rows, s);
+  if (rows >= 8 * sms && packs <= 1024) return launch_c<T, V, 32, 1, TOP>(a, rows, s);
+  if (packs <= 256 || (rows >= sms && packs <= 4096)) return launch_c<T, V, 128, 1, TOP>(a, rows, s);
   int c = 1;
   while (c < 8 && rows * c < 2 * sms && packs >= 512 * 2 * c) c *= 2;
   switch (c) {
