@@ -130,6 +130,7 @@ APPY_DEV unsigned in_block(unsigned address, int rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
   return r;
 }
+
 // V channels per thread, CP threads along the channels, LT tokens per thread, NT threads, C blocks per cluster.
 //
 // Where rows start on 16-byte boundaries, TMA brings the tiles of a step (L tokens of CH channels of each array) into a

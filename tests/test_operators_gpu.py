@@ -619,6 +619,8 @@ def test_refusals(rt):
             (ValueError, lambda: appy.embedding(w, tokens, out=randn(4, 7))), (ValueError, lambda: appy.embedding(w, tokens, out=randn(4, 8).half())),
             (ValueError, lambda: appy.embedding(w, tokens, out=randn(8, 4).t())), (TypeError, lambda: appy.embedding(w, np.zeros(4, np.int64))),
             (ValueError, lambda: appy.embedding(w, tokens, out=randn(1, 8).expand(4, 8))), (TypeError, lambda: appy.embedding([1.0], tokens)),
+            (ValueError, lambda: appy.embedding(w, tokens.cpu())), (ValueError, lambda: appy.gated_scan(x, x, randn(2, 8).cpu())),
+            (ValueError, lambda: appy.token_logprobs_grad(logits, tokens, randn(4, 3).cpu())),
             (ValueError, lambda: appy.embedding_grad(randn(4, 8), tokens)), (ValueError, lambda: appy.embedding_grad(randn(3, 8), tokens, 10)),
             (ValueError, lambda: appy.embedding_grad(randn(4, 8), tokens, 10, accumulate=True)),
             (ValueError, lambda: appy.embedding_grad(randn(4, 8), tokens, 10, out=randn(9, 8))),
