@@ -120,7 +120,7 @@ def draw_tokens(kind, n, rows, seed):
 
 @pytest.mark.parametrize("dtype, out_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
                                               (torch.bfloat16, torch.float32), (torch.float16, torch.float32)])
-@pytest.mark.parametrize("n, rows, width", [(1, 1, 1), (1, 1000, 64), (31, 5, 8), (33, 511, 769), (700, 512, 100), (4096, 513, 256), (4097, 100, 40),
+@pytest.mark.parametrize("n, rows, width", [(1, 1, 1), (1, 1000, 64), (31, 5, 8), (33, 511, 769), (256, 90, 24), (257, 90, 24), (700, 512, 100), (4096, 513, 256), (4097, 100, 40),
                                             (9000, 70001, 72), (20011, 300, 264)])
 def test_embedding_grad(rt, dtype, out_dtype, n, rows, width):
     for k, kind in enumerate(["uniform", "zipf", "one", "two", "none", "falling"]):
