@@ -46,24 +46,17 @@ template <class T, int V> struct Pack {
     APPY_DEV Bits() {}
   };
 };
-template <class R> APPY_DEV R ld_raw_cs(const R* p) { return __ldcs(p); }
-APPY_DEV Raw32 ld_raw_cs(const Raw32* p) { return {__ldcs(&p->a), __ldcs(&p->b)}; }
-template <class R> APPY_DEV R ld_raw_nc(const R* p) { return __ldg(p); }
-APPY_DEV Raw32 ld_raw_nc(const Raw32* p) { return {__ldg(&p->a), __ldg(&p->b)}; }
-template <class R> APPY_DEV void st_raw_cs(R* p, const R& v) { __stcs(p, v); }
-APPY_DEV void st_raw_cs(Raw32* p, const Raw32& v) { __stcs(&p->a, v.a); __stcs(&p->b, v.b); }
-
 template <class T, int V> APPY_DEV Pack<T, V> ld_stream(const T* p) {        // read once: evict-first
-  return {ld_raw_cs(reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p))};
+  return {__ldcs(reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p))};
 }
 template <class T, int V> APPY_DEV Pack<T, V> ld_keep(const T* p) {          // read again soon, never written here
-  return {ld_raw_nc(reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p))};
+  return {__ldg(reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p))};
 }
 template <class T, int V> APPY_DEV Pack<T, V> ld_plain(const T* p) {         // this kernel may also write there
   return {*reinterpret_cast<const typename Raw<sizeof(T) * V>::type*>(p)};
 }
 template <class T, int V> APPY_DEV void st_stream(T* p, Pack<T, V> v) {
-  st_raw_cs(reinterpret_cast<typename Raw<sizeof(T) * V>::type*>(p), v.raw);
+  __stcs(reinterpret_cast<typename Raw<sizeof(T) * V>::type*>(p), v.raw);
 }
 template <class T, int V> APPY_DEV void st_plain(T* p, Pack<T, V> v) {
   *reinterpret_cast<typename Raw<sizeof(T) * V>::type*>(p) = v.raw;
