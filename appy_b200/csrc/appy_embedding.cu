@@ -28,7 +28,7 @@ APPY_DEV i64 token_of(const void* tokens, bool wide, i64 n) {
 
 // ------------------------------------------------------------------------------------------------ lookup
 // Rows of at least 32 packs: a warp takes a stretch of one row, so that no pack needs an index of its own (65536 rows
-// of 4096 bfloat16: the flat form issued 118 instructions per 32 packs, four fifths of all issue slots).  Shorter
+// of 4096 bfloat16 121 us; the flat form, at 118 instructions per 32 packs, four fifths of all issue slots, 144).  Shorter
 // rows: flat over the packs of the output, pack i of row i / per_row; neighbouring threads read one row, so token
 // loads are broadcasts.
 const int kLookupBlock = 256;
