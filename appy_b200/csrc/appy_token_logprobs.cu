@@ -7,10 +7,11 @@
 // One pass over the row: every thread keeps its own m, S and Q and rescales them when its maximum grows.  S and Q
 // are float32 sums of at most a few hundred terms per thread, joined as a tree.
 //
-// Masked logits may be -inf or the type's lowest value, and products with k may leave the float32 range there.  d is
-// therefore held above -1000, where its weight has long been zero, and a row whose maximum itself lies that far out
-// (to either side) takes x - m first (see `Scaled`).  A row of -inf only is empty: log probability -inf,
-// entropy 0, no gradient.  A row with a NaN or +inf is NaN throughout.
+// Masked logits may be -inf, the type's lowest value, or any large finite one.  The fused form of d takes the rounded product
+// m k for the reference, which at x = m is off by up to half a step of that product, so it is used where this is at most a
+// quarter; a row (or a thread's part of it) whose maximum lies farther out takes x - m first (see `Scaled`).  d is held above
+// -1000, where its weight has long been zero.  A row of -inf only is empty: log probability -inf, entropy 0, no gradient.  A
+// row with a NaN or +inf is NaN throughout.
 //
 // Top alternatives: a thread remembers its best pack.  The `top`-th largest of 64 groups' bests bounds the answer
 // from below, so only packs not below it are looked at again, and the few elements found are ranked by
@@ -40,12 +41,13 @@ APPY_DEV float max_nan(float a, float b) {               // NaN if either is
   return r;
 }
 
-// k and a bound: a maximum within +-limit stays within float32 when multiplied by k
+// k and a bound: a maximum within +-limit has a product with k below 2^22, whose half step is at most 2^-2
 struct Scale { float k, limit, span, inv_temperature; };      // span: 2^(-span k) is below float32
 
 // d = (x - m) * k.  For a maximum within the limit as one fused multiply-add against the rounded product m * k: that product is a
 // reference like any other, as long as every use of this m has the same one (so it must not be contracted into a
-// difference of two of them).
+// difference of two of them).  Beyond it the maximum itself is the reference: at x = m the fused form would give the rounding
+// of the product, 439 for m = -1e10 and 6e21 for -1e30 at temperature 1, and its weight would be infinite or zero.
 struct Scaled {
   float m, mk;
   bool far;                                              // maximum beyond the limit (or no maximum yet)
@@ -65,7 +67,11 @@ struct Part {
 APPY_DEV Part rescaled(const Part& p, float m, const Scale& s) {
   if (p.s == 0.f) return {m, 0.f, 0.f};
   const Scaled now(m, s), was(p.m, s);
-  const float d = now.far ? fmaxf((p.m - m) * s.k, -1000.f) : was.far ? -1000.f : was.mk - now.mk, c = exp2_fast(d);
+  // the old reference against the new: each is its maximum times k, rounded (within the limit) or not
+  float d = was.mk - now.mk;
+  if (__builtin_expect(now.far || was.far, 0)) d = !was.far ? -fmaf(m, s.k, -was.mk) : now.far ? (p.m - m) * s.k : fmaf(p.m, s.k, -now.mk);
+  d = fmaxf(d, -1000.f);
+  const float c = exp2_fast(d);
   return {m, p.s * c, c * (p.q + p.s * d)};
 }
 APPY_DEV Part joined(const Part& a, const Part& b, const Scale& s) {
@@ -150,7 +156,7 @@ template <class T> APPY_DEV bool bound_of(const Scaled& d, const Scale& s, unsig
     const unsigned short h = __half_as_ushort(__float2half_rd(b));
     bound = h | (unsigned)h << 16;
   }
-  return fabsf(d.m) <= s.span * 65536.f && !d.far;             // else m - span may be m
+  return !d.far;                                         // else m - span may be m
 }
 
 // One thread's part of a row: softmax with its own maximum, S and Q as pairs of sums.
@@ -590,7 +596,7 @@ template <class T, bool TOP> int launch_logprobs(const LogprobArgs& a, i64 rows,
 
 Scale scale_of(float temperature) {
   const float k = 1.44269504088896341f / temperature;
-  return {k, 1e38f / (k > 1.f ? k : 1.f), 200.f / k, 1.f / temperature};
+  return {k, 4194304.f / k, 200.f / k, 1.f / temperature};
 }
 
 int check_logits(const char* fn, int dtype, int token_dtype, i64 rows, i64 cols, i64 ld, float temperature) {

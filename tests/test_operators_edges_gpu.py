@@ -1,0 +1,38 @@
+"""The language-model operators at the edges of what they accept: values, aliases and callers that ordinary use does not reach."""
+import pytest
+
+import appy_b200 as appy
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_operators_gpu import check_logprobs, gen, randn  # noqa: E402
+
+
+# ------------------------------------------------------------------------------------------------ log probabilities
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-1e9, -1e10, -1e20, -1e30, -1e37])
+@pytest.mark.parametrize("temperature", [0.5, 0.6, 0.7, 0.8, 1.0, 2.0])
+def test_token_logprobs_masked_by_large_finite_values(rt, dtype, mask, temperature):
+    """Every distance from a logit to the row's maximum is taken from the maximum itself where the product of the maximum
+    and log2(e) / temperature would be rounded by more than a fraction of one: the bounds are those of any other row."""
+    for cols in (37, 3001, 20000):
+        wide = randn(9, cols + 1, dtype=dtype, seed=cols, std=2.0)
+        for logits in (wide[:, :cols], wide[:, 1:]):             # rows on 16 bytes or not, and all off them
+            logits[0] = mask                                     # nothing else
+            logits[1, cols // 2:] = mask                         # a padded vocabulary's tail
+            logits[2, : cols // 2] = mask
+            logits[3] = mask
+            logits[3, cols // 3] = 1.5                           # one left
+            logits[4, 0] = mask
+            logits[5, ::2] = mask
+            logits[6] = -mask                                    # large and positive
+            logits[7, cols - 1] = -mask
+            logits[8] = mask
+            logits[8, 0] = 2 * mask                              # two kinds
+            logits[8, cols - 1] = mask * 0.75
+            tokens = torch.randint(0, cols, (9,), generator=gen(2), device="cuda")
+            tokens[1], tokens[2], tokens[3] = 3, cols - 1, cols // 3
+            check_logprobs(logits, tokens, temperature, min(20, cols))
+    check_logprobs(torch.cat([logits] * 40), torch.cat([tokens] * 40), temperature, 5)
