@@ -743,6 +743,10 @@ template <class T, class O, int V> int launch_sums(const SumArgs& a, const T* g,
   return finish("embedding gradient sum launch");
 }
 
+// Positions, rows and keys are int on the device: the end of the last share or tile, and the 64 positions that a warp looks ahead,
+// must not pass 2^31.
+bool grad_sizes(i64 n, i64 rows, i64 width) { return n >= 0 && n <= 0x7fff0000 && rows >= 0 && rows < 0x7fffffff && width >= 0; }
+
 int grad_vec(const void* g, int dtype, i64 ldg, const void* out, int out_dtype, i64 ldo, i64 width) {
   // one pack per thread and position: 8 16-bit columns or 4 float32 ones, if rows start where such packs may
   const int V = dtype == APPY_F32 ? 4 : 8, so = element_size(out_dtype);
@@ -790,7 +794,7 @@ int appy_embedding(const void* dweight, int dtype, int64_t ldw, int64_t rows, in
 int appy_embedding_grad_bytes(int64_t n, int64_t rows, int64_t width, size_t* bytes) {
   static const char fn[] = "appy_embedding_grad_bytes";
   if (!bytes) return fail_named(fn, "NULL argument");
-  if (rows < 0 || width < 0 || n < 0 || n >= 0x7fffffff || rows >= 0x7fffffff) return fail_named(fn, "sizes must be in [0, 2^31 - 1)");
+  if (!grad_sizes(n, rows, width)) return fail_named(fn, "sizes must not be negative, n at most 2^31 - 2^16, rows below 2^31 - 1");
   size_t most = 0;
   for (int vec : {1, 4, 8}) most = std::max(most, grad_plan(n, rows, width, vec).bytes);
   *bytes = std::max<size_t>(most, 256);
@@ -804,7 +808,7 @@ int appy_embedding_grad(const void* dgrad, int dtype, int64_t ldg, const void* d
   if (!element_size(dtype)) return fail_named(fn, "dtype must be APPY_F32, APPY_F16 or APPY_BF16");
   if (out_dtype != dtype && out_dtype != APPY_F32) return fail_named(fn, "out_dtype must be dtype or APPY_F32");
   if (token_dtype != APPY_I32 && token_dtype != APPY_I64) return fail_named(fn, "token_dtype must be APPY_I32 or APPY_I64");
-  if (rows < 0 || width < 0 || n < 0 || n >= 0x7fffffff || rows >= 0x7fffffff) return fail_named(fn, "sizes must be in [0, 2^31 - 1)");
+  if (!grad_sizes(n, rows, width)) return fail_named(fn, "sizes must not be negative, n at most 2^31 - 2^16, rows below 2^31 - 1");
   if (rows == 0 || width == 0) return APPY_OK;
   if (!dout || (n && (!dgrad || !dtokens || !dworkspace))) return fail_named(fn, "NULL argument");
   if (ldg < width || ldo < width) return fail_named(fn, "ldg and ldo must be at least width");

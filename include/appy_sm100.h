@@ -245,8 +245,9 @@ int appy_embedding(const void* dweight, int dtype, int64_t ldw, int64_t rows, in
                    void* stream);
 /* out[v,:] = scale * sum of grad[n,:] over all n with tokens[n] == v, for v < rows; with accumulate != 0 the sum is
  * added to out, and rows without tokens are left as they are.  Tokens outside [0, rows) are dropped.  The sum of a
- * row runs in float32 over its positions sorted.  out_dtype is dtype or APPY_F32.  `dworkspace` holds at least
- * appy_embedding_grad_bytes(...) bytes, aligned to 256; its contents before and after do not matter. */
+ * row runs in float32 over its positions sorted.  n is at most 2^31 - 2^16.  out_dtype is dtype or APPY_F32.
+ * `dworkspace` holds at least appy_embedding_grad_bytes(...) bytes, aligned to 256; its contents before and after do
+ * not matter. */
 int appy_embedding_grad_bytes(int64_t n, int64_t rows, int64_t width, size_t* bytes);
 int appy_embedding_grad(const void* dgrad, int dtype, int64_t ldg, const void* dtokens, int token_dtype, int64_t n,
                         int64_t rows, int64_t width, float scale, int accumulate, void* dout, int out_dtype,

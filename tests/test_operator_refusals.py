@@ -108,3 +108,11 @@ def test_nothing_to_do_is_no_error():
     for name, *args in (embedding(n=0, tokens=N, out=N), embedding(width=0), grad(rows=0), grad(width=0), scan(sequences=0), scan(width=0),
                         scan_grad(sequences=0), logprobs(rows=0), logprobs_grad(rows=0)):
         assert getattr(lib, name)(*args, None) == 0
+
+
+@pytest.mark.parametrize("n", [(1 << 31) - 2, (1 << 31) - 1024, (1 << 31) - (1 << 16) + 1])
+def test_embedding_grad_of_positions_whose_shares_would_pass_32_bits(n):
+    size = C.c_size_t()
+    assert "sizes" in refused(*grad(n=n, size=1 << 40))
+    assert rt.lib().appy_embedding_grad_bytes(n, 10, 8, C.byref(size)) == -3
+    assert rt.lib().appy_embedding_grad_bytes((1 << 31) - (1 << 16), 10, 8, C.byref(size)) == 0
