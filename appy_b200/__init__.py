@@ -24,19 +24,23 @@ import textwrap
 from . import dispatcher
 from .frontend.static_rewrite import RUNTIME_NAME, rewrite_function_source
 
-__all__ = ["jit", "prange", "range", "vidx", "to_gpu", "to_cpu", "shader", "cpu_shader", "set_default_options",
-           "embedding", "embedding_grad", "gated_scan", "gated_scan_grad", "token_logprobs", "token_logprobs_grad"]
+__all__ = ["jit", "prange", "range", "vidx", "to_gpu", "to_cpu", "shader", "cpu_shader", "set_default_options"]
 
-_OPERATORS = frozenset(__all__[-6:])
+# Names of the language-model operators (operators.py).  They need torch, which is imported with the first of them that is
+# asked for: not with this package, and not by a star import, which takes every name of __all__.
+_OPERATORS = ("embedding", "embedding_grad", "gated_scan", "gated_scan_grad", "token_logprobs", "token_logprobs_grad")
 
 
 def __getattr__(name):
-    """The language-model operators (operators.py) need torch, which is imported with the first of them."""
     if name in _OPERATORS:
         from . import operators
         globals().update({n: getattr(operators, n) for n in _OPERATORS})
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted(set(globals()) | set(_OPERATORS))
 
 
 _builtin_range = range
