@@ -422,18 +422,13 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     device = _together(fn, logits, tokens)
     logits, ld = _rows_in(logits)
     tokens = tokens.contiguous()
-    shape, n, dev = tokens.shape, tokens.numel(), logits.device
-    # one allocation for the float32 results: an allocation costs the host more than a view
-    logprobs, entropy, stats, top_logprobs = torch.empty(n * (5 + top), dtype=torch.float32, device=dev).split((n, n, 3 * n, top * n))
-    stats = stats.view(shape + (3,))
-    if len(shape) != 1:
-        logprobs, entropy = logprobs.view(shape), entropy.view(shape)
-    top_tokens = None
+    shape, n = tokens.shape, tokens.numel()
+    # arrays of their own: pieces of one allocation would be views, which autograd does not let a caller write in place
+    logprobs = logits.new_empty(shape, dtype=torch.float32)
+    entropy, stats = torch.empty_like(logprobs), logprobs.new_empty(shape + (3,))
+    top_logprobs = top_tokens = None
     if top:
-        top_logprobs = top_logprobs.view(shape + (top,))
-        top_tokens = torch.empty(shape + (top,), dtype=tokens.dtype, device=dev)
-    else:
-        top_logprobs = None
+        top_logprobs, top_tokens = logprobs.new_empty(shape + (top,)), tokens.new_empty(shape + (top,))
     _run("appy_token_logprobs", device, logits.data_ptr(), code, ld, n, cols, tokens.data_ptr(), int_code, float(temperature), top,
          logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr(), _ptr(top_logprobs), _ptr(top_tokens))
     return LogProbs(logprobs, entropy, stats, top_logprobs, top_tokens)

@@ -6,7 +6,7 @@ import appy_b200 as appy
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_operators_gpu import check_logprobs, gen, randn  # noqa: E402
+from test_operators_gpu import TokenLogprobs, check_logprobs, gen, randn  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ log probabilities
@@ -36,3 +36,20 @@ def test_token_logprobs_masked_by_large_finite_values(rt, dtype, mask, temperatu
             tokens[1], tokens[2], tokens[3] = 3, cols - 1, cols // 3
             check_logprobs(logits, tokens, temperature, min(20, cols))
     check_logprobs(torch.cat([logits] * 40), torch.cat([tokens] * 40), temperature, 5)
+
+
+def test_results_of_log_probabilities_are_arrays_of_their_own(rt):
+    logits, tokens = randn(6, 50, seed=1).requires_grad_(), torch.arange(6, device="cuda")
+    lp, entropy = TokenLogprobs.apply(logits, tokens)
+    keep = (tokens % 2 == 0).float()
+    lp.mul_(keep)                                                # in place, as a loss over a padded batch does it
+    entropy.masked_fill_(keep == 0, 0.0)
+    (lp.sum() + entropy.sum()).backward()
+    r = appy.token_logprobs(logits.detach(), tokens, top=3)
+    assert torch.equal(logits.grad, appy.token_logprobs_grad(logits.detach(), tokens, r.stats, keep, keep))
+    stats = r.stats.clone()
+    before = r.stats._version
+    r.logprobs.zero_(), r.entropy.zero_(), r.top_logprobs.zero_()
+    assert torch.equal(r.stats, stats) and r.stats._version == before
+    for v in r:
+        assert not v._is_view() and v.untyped_storage().nbytes() == v.numel() * v.element_size()
