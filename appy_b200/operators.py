@@ -10,11 +10,11 @@ with annotated loops.  Element types are float32, float16 and bfloat16; arithmet
 once.  Token and offset arrays are int32 or int64.  Inputs may have any strides (a layout that the kernels do not read
 in place, such as a transposed last dimension, is copied first); arrays that are written need a unit last stride.
 
-Gradients are functions of their own: nothing is recorded for autograd, and a tensor that requires grad is refused
-while grad mode is on.  A ``torch.autograd.Function`` whose ``forward`` calls ``f`` and whose ``backward`` calls
-``f_grad`` puts an operator into a graph.  Calls may be captured into CUDA graphs, gradients included, once each kind of
-call has run outside of one (kernels are loaded with their first call).  An array that is written must not overlap an
-argument, unless it says so.
+Gradients are functions of their own: nothing is recorded for autograd; a tensor that requires grad is refused while
+grad mode is on, and one that carries a forward-mode tangent.  A ``torch.autograd.Function`` whose ``forward`` calls
+``f`` and whose ``backward`` calls ``f_grad`` puts an operator into a graph.  Calls may be captured into CUDA graphs,
+gradients included, once each kind of call has run outside of one (kernels are loaded with their first call).  An array
+that is written must not overlap an argument, unless it says so.
 """
 from __future__ import annotations
 
@@ -23,6 +23,7 @@ from collections import namedtuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .backends.cuda_sm100 import runtime as rt
 
@@ -100,7 +101,7 @@ def _ints(fn, name, t):
 
 
 def _together(fn, first, *others):
-    """All on the device of `first`, none of them part of an autograd graph."""
+    """All on the device of `first`, none of them part of an autograd graph, backwards or forwards."""
     device = first.device
     grad = torch.is_grad_enabled()
     if grad and first.requires_grad:
@@ -112,6 +113,11 @@ def _together(fn, first, *others):
             _fail(fn, f"arguments are on {device} and {t.device}")
         if grad and t.requires_grad:
             _no_graph(fn)
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in (first, *others):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{fn}: an argument carries a forward-mode tangent, but autograd does not see this operator: "
+                                   "call it on primal values, or inside a torch.autograd.Function that has a jvp")
     return device.index
 
 

@@ -53,3 +53,23 @@ def test_results_of_log_probabilities_are_arrays_of_their_own(rt):
     assert torch.equal(r.stats, stats) and r.stats._version == before
     for v in r:
         assert not v._is_view() and v.untyped_storage().nbytes() == v.numel() * v.element_size()
+
+
+# ------------------------------------------------------------------------------------------------ autograd
+
+def test_forward_mode_is_refused(rt):
+    import torch.autograd.forward_ad as fwad
+    w, tokens, x, logits = randn(10, 8, seed=1), torch.arange(4, device="cuda"), randn(2, 5, 8, seed=2), randn(4, 8, seed=3)
+    h, _ = appy.gated_scan(x, x)
+    stats = appy.token_logprobs(logits, tokens).stats
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in [lambda: appy.embedding(dual(w), tokens), lambda: appy.embedding_grad(dual(logits), tokens, 10), lambda: appy.gated_scan(x, dual(x)),
+                     lambda: appy.gated_scan(x, x, dual(x[:, 0].contiguous())), lambda: appy.gated_scan_grad(dual(x), x, x, h),
+                     lambda: appy.token_logprobs(dual(logits), tokens), lambda: appy.token_logprobs_grad(dual(logits), tokens, stats),
+                     lambda: appy.embedding(dual(w.cpu()), tokens.cpu())]:
+            before = rt.launch_count()
+            with pytest.raises(RuntimeError, match="autograd"):
+                call()
+            assert rt.launch_count() == before
+        assert torch.equal(appy.embedding(w, tokens), w[tokens])         # without a tangent it goes on as ever
