@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kLookupBlock) k_lookup_rows(const T* __restric
       k[u] = zero_pack<T, V>();
       if (known && c + 32 * u < count) k[u] = ld_keep<T, V>(from + (c + 32 * u) * V);
     }
-    if (scale != 1.f) {
+    if (scale != 1.f && known) {                   // the zeros of an unknown token stay +0 whatever the scale
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float f[V];

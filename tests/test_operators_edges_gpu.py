@@ -1,4 +1,6 @@
 """The language-model operators at the edges of what they accept: values, aliases and callers that ordinary use does not reach."""
+import math
+
 import pytest
 
 import appy_b200 as appy
@@ -6,7 +8,7 @@ import appy_b200 as appy
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_operators_gpu import TokenLogprobs, check_logprobs, gen, randn  # noqa: E402
+from test_operators_gpu import TYPES, TokenLogprobs, check_logprobs, gen, randn  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ log probabilities
@@ -73,3 +75,17 @@ def test_forward_mode_is_refused(rt):
                 call()
             assert rt.launch_count() == before
         assert torch.equal(appy.embedding(w, tokens), w[tokens])         # without a tangent it goes on as ever
+
+
+# ------------------------------------------------------------------------------------------------ embedding
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [8, 100, 769, 1024])
+@pytest.mark.parametrize("scale", [-2.0, math.inf, -math.inf, math.nan])
+def test_unknown_tokens_give_positive_zeros_whatever_the_scale(rt, dtype, width, scale):
+    w = randn(20, width, dtype=dtype, seed=1)
+    tokens = torch.tensor([-1, 3, 20, 7, 1 << 40, -(1 << 40)], device="cuda")
+    got = appy.embedding(w, tokens, scale=scale)
+    unknown = got[[0, 2, 4, 5]]
+    assert not unknown.any() and not torch.signbit(unknown).any()
+    assert torch.equal(got[[1, 3]].nan_to_num(7.0), (w[[3, 7]].float() * scale).to(dtype).nan_to_num(7.0))
