@@ -8,7 +8,7 @@ import appy_b200 as appy
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_operators_gpu import TYPES, TokenLogprobs, check_logprobs, gen, randn  # noqa: E402
+from test_operators_gpu import TYPES, TokenLogprobs, check_logprobs, gen, grad_reference, grad_tolerance, randn, within  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ log probabilities
@@ -89,3 +89,50 @@ def test_unknown_tokens_give_positive_zeros_whatever_the_scale(rt, dtype, width,
     unknown = got[[0, 2, 4, 5]]
     assert not unknown.any() and not torch.signbit(unknown).any()
     assert torch.equal(got[[1, 3]].nan_to_num(7.0), (w[[3, 7]].float() * scale).to(dtype).nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("n", [5, 300])
+@pytest.mark.parametrize("width", [8, 7])
+def test_embedding_grad_accumulates_subnormal_values(rt, n, width):
+    small = 2.0 ** -140
+    out = torch.full((4, width), small, device="cuda")
+    tokens = torch.full((n,), 2, device="cuda")
+    grad = torch.zeros(n, width, device="cuda")
+    appy.embedding_grad(grad, tokens, out=out, accumulate=True)
+    assert (out == small).all()                                  # zeros added
+    grad[0] = 3 * small
+    appy.embedding_grad(grad, tokens, out=out, accumulate=True)
+    assert (out[2] == 4 * small).all() and (out[[0, 1, 3]] == small).all()
+
+
+@pytest.mark.parametrize("n", [200, 700])
+@pytest.mark.parametrize("width", [64, 61])
+def test_embedding_grad_accumulates_with_one_rounding_down_to_the_smallest_values(rt, n, width):
+    """Every row has one position: the result is the sum of two float32 numbers, rounded once."""
+    gradient = torch.randn(n, width, generator=gen(1), device="cuda") * 2.0 ** torch.randint(-149, -99, (n, width), generator=gen(2), device="cuda").double()
+    old = torch.randn(n, width, generator=gen(3), device="cuda") * 2.0 ** torch.randint(-149, -99, (n, width), generator=gen(4), device="cuda").double()
+    gradient, old = gradient.float(), old.float()
+    old[:, ::5] = -gradient[:, ::5] * (1 + 2.0 ** -20)           # nearly cancelling
+    gradient[: n // 2] = torch.where(gradient[: n // 2].abs() < 2.0 ** -101, 2.0 ** -101, gradient[: n // 2])      # the other way of adding
+    tokens = torch.randperm(n, generator=gen(5), device="cuda")
+    out = old.clone()
+    appy.embedding_grad(gradient, tokens, out=out, accumulate=True)
+    want = (old[tokens].double() + gradient.double()).float()    # 2^-149 to 2^-96: exact in 64 bits, then rounded
+    assert torch.equal(out[tokens], want)
+
+
+@pytest.mark.parametrize("dtype, out_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32), (torch.float32, torch.float32),
+                                              (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("n", [40, 256, 257, 3000])
+@pytest.mark.parametrize("width", [64, 67, 1])
+def test_embedding_grad_accumulates_in_every_form(rt, dtype, out_dtype, n, width):
+    rows = 90
+    tokens = torch.randint(-2, rows + 2, (n,), generator=gen(n), device="cuda")
+    tokens[: n // 3] = 5                                         # one frequent row
+    grad, out = randn(n, width, dtype=dtype, seed=1), randn(rows, width, dtype=out_dtype, seed=2)
+    before = out.clone()
+    got = appy.embedding_grad(grad, tokens, scale=-0.5, out=out, accumulate=True)
+    ref, size, count = grad_reference(grad, tokens, rows, -0.5)
+    assert got is out
+    within(out, ref + before.double(), grad_tolerance(ref + before.double(), size + before.double().abs(), count + 1, out_dtype))
+    assert torch.equal(out[count[:, 0] == 0], before[count[:, 0] == 0])
