@@ -650,6 +650,15 @@ int check_shape(const char* fn, int dtype, const void* offsets, int offsets_dtyp
   return APPY_OK;
 }
 
+// Of no sequences at all, every packed row is one of no sequence.
+int clear_all(const char* fn, void* p, i64 row, int dtype, i64 tokens, i64 width, void* stream) {
+  if (tokens == 0) return APPY_OK;
+  if (!p) return fail_named(fn, "NULL argument");
+  const size_t size = (size_t)element_size(dtype);
+  const cudaError_t e = cudaMemset2DAsync(p, (size_t)row * size, 0, (size_t)width * size, (size_t)tokens, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? APPY_OK : appy_fail_cuda(e, "gated scan clear");
+}
+
 }  // namespace
 
 extern "C" {
@@ -659,7 +668,8 @@ int appy_gated_scan(const void* dx, int64_t x_seq, int64_t x_row, const void* dg
                     const float* dinitial, void* dh, int64_t h_seq, int64_t h_row, float* dlast, int fill, void* stream) {
   static const char fn[] = "appy_gated_scan";
   if (int rc = check_shape(fn, dtype, doffsets, offsets_dtype, sequences, tokens, width)) return rc;
-  if (sequences == 0 || width == 0) return APPY_OK;
+  if (width == 0) return APPY_OK;
+  if (sequences == 0) return fill && doffsets ? clear_all(fn, dh, h_row, dtype, tokens, width, stream) : APPY_OK;
   if (tokens && (!dx || !dgate || !dh)) return fail_named(fn, "NULL argument");
   ScanArgs a = {};
   a.x = {const_cast<void*>(dx), x_seq, x_row};
@@ -684,7 +694,12 @@ int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const 
                          void* dgrad_gate, int64_t gg_seq, int64_t gg_row, float* dgrad_initial, int fill, void* stream) {
   static const char fn[] = "appy_gated_scan_grad";
   if (int rc = check_shape(fn, dtype, doffsets, offsets_dtype, sequences, tokens, width)) return rc;
-  if (sequences == 0 || width == 0) return APPY_OK;
+  if (width == 0) return APPY_OK;
+  if (sequences == 0) {
+    if (!fill || !doffsets) return APPY_OK;
+    const int rc = clear_all(fn, dgrad_x, gx_row, dtype, tokens, width, stream);
+    return rc ? rc : clear_all(fn, dgrad_gate, gg_row, dtype, tokens, width, stream);
+  }
   if (tokens && (!dx || !dgate || !dh || !dgrad_x || !dgrad_gate)) return fail_named(fn, "NULL argument");
   ScanArgs a = {};
   a.dh = {const_cast<void*>(ddh), dh_seq, dh_row};

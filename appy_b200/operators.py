@@ -355,8 +355,6 @@ def gated_scan(x, gate, initial=None, offsets=None, out=None, last=None):
         if not last.is_contiguous():
             _fail(fn, "last must be contiguous")
     device = _together(fn, x, gate, initial, offsets, out, last)
-    if fill and sequences == 0:
-        out.zero_()
     _run("appy_gated_scan", device, *_strided(x), *_strided(gate), code, _ptr(offsets), int_code, sequences, tokens, x.shape[-1],
          _ptr(initial), *_strided(out), last.data_ptr(), fill)
     return out, last
@@ -391,8 +389,6 @@ def gated_scan_grad(grad, x, gate, h, initial=None, offsets=None, grad_last=None
         _scan_out(fn, "out[1]", dgate, x)
     dinitial = torch.empty(shape, dtype=torch.float32, device=x.device)
     device = _together(fn, x, gate, h, grad, initial, offsets, grad_last, dx, dgate)
-    if fill and sequences == 0:
-        dx.zero_(), dgate.zero_()
     _run("appy_gated_scan_grad", device, *(_strided(grad) if grad is not None else (None, 0, 0)), *_strided(x), *_strided(gate), *_strided(h),
          code, _ptr(offsets), int_code, sequences, tokens, x.shape[-1], _ptr(initial), _ptr(grad_last), *_strided(dx), *_strided(dgate),
          dinitial.data_ptr(), fill)

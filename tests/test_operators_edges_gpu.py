@@ -136,3 +136,30 @@ def test_embedding_grad_accumulates_in_every_form(rt, dtype, out_dtype, n, width
     assert got is out
     within(out, ref + before.double(), grad_tolerance(ref + before.double(), size + before.double().abs(), count + 1, out_dtype))
     assert torch.equal(out[count[:, 0] == 0], before[count[:, 0] == 0])
+
+
+# ------------------------------------------------------------------------------------------------ gated recurrence
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_no_sequence_are_cleared_for_no_sequences_too(rt, dtype):
+    x = randn(9, 24, dtype=dtype, seed=1)
+    out = [torch.full((9, 40), 7.0, dtype=dtype, device="cuda") for _ in range(3)]
+    offsets = torch.zeros(1, dtype=torch.int32, device="cuda")
+    code = {torch.float32: 0, torch.float16: 4, torch.bfloat16: 5}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def place(t):
+        return t.data_ptr(), 0, t.stride(0)
+
+    def call(fill):
+        rt.check(rt.lib().appy_gated_scan(*place(x), *place(x), code, offsets.data_ptr(), 2, 0, 9, 24, None, *place(out[0]), None, fill, stream))
+        rt.check(rt.lib().appy_gated_scan_grad(*place(x), *place(x), *place(x), *place(x), code, offsets.data_ptr(), 2, 0, 9, 24, None, None,
+                                               *place(out[1]), *place(out[2]), None, fill, stream))
+
+    call(0)
+    assert all((o == 7).all() for o in out)
+    call(1)
+    assert all(not o[:, :24].any() and (o[:, 24:] == 7).all() for o in out)
+    h, last = appy.gated_scan(x, x, offsets=offsets)
+    dx, dg, d0 = appy.gated_scan_grad(x, x, x, h, offsets=offsets)
+    assert not h.any() and not dx.any() and not dg.any() and last.shape == d0.shape == (0, 24)
