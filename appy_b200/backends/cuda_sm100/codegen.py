@@ -1193,6 +1193,14 @@ def touch(*arrays):
             st[1] = False
 
 
+def touch_bytes(lo: int, hi: int) -> None:
+    """Host memory in [lo, hi) was written: `touch` for every resident array that has part of it, by whatever name it
+    was written."""
+    for p, st in _resident.items():
+        if p < hi and lo < p + st[0]:
+            st[1] = False
+
+
 def release(*arrays):
     for a in arrays:
         _resident.pop(_host_base(a), None)

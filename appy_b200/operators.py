@@ -42,6 +42,16 @@ def _is_host(a) -> bool:
     return not (isinstance(a, torch.Tensor) and a.is_cuda)
 
 
+def _touch(h):
+    """A host array was written here: loops that keep it on the device upload it again."""
+    from .backends.cuda_sm100 import codegen
+    if isinstance(h, np.ndarray):
+        codegen.touch_bytes(*np.lib.array_utils.byte_bounds(h))
+    else:
+        lo = h.untyped_storage().data_ptr()
+        codegen.touch_bytes(lo, lo + h.untyped_storage().nbytes())
+
+
 def _through_host(fn, args, kwargs):
     """Run `fn` on uploaded copies of host arguments and bring results (and written arguments) back."""
     from . import to_gpu
@@ -64,6 +74,7 @@ def _through_host(fn, args, kwargs):
         for h, d in pairs:
             if h is not None and h is not d:
                 (torch.from_numpy(h) if isinstance(h, np.ndarray) else h).copy_(d)
+                _touch(h)
                 written[id(d)] = h
 
     def down(t):

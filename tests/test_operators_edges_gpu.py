@@ -1,6 +1,7 @@
 """The language-model operators at the edges of what they accept: values, aliases and callers that ordinary use does not reach."""
 import math
 
+import numpy as np
 import pytest
 
 import appy_b200 as appy
@@ -163,3 +164,35 @@ def test_rows_of_no_sequence_are_cleared_for_no_sequences_too(rt, dtype):
     h, last = appy.gated_scan(x, x, offsets=offsets)
     dx, dg, d0 = appy.gated_scan_grad(x, x, x, h, offsets=offsets)
     assert not h.any() and not dx.any() and not dg.any() and last.shape == d0.shape == (0, 24)
+
+
+# ------------------------------------------------------------------------------------------------ host arrays
+
+@appy.jit
+def doubled(a, out):
+    #pragma parallel for
+    for i in range(out.shape[0]):
+        #pragma simd
+        for j in range(out.shape[1]):
+            out[i, j] = a[i, j] * 2.0
+    return out
+
+
+def test_loops_see_what_an_operator_wrote_to_a_resident_array(rt):
+    rng = np.random.default_rng(0)
+    w, tokens = rng.standard_normal((20, 12), dtype=np.float32), rng.integers(0, 20, 30)
+    whole = np.ones((40, 12), np.float32)
+    appy.resident(whole)
+    try:
+        out = np.empty_like(whole)
+        doubled(whole, out)
+        assert np.array_equal(out, 2 * whole)
+        appy.embedding(w, tokens, out=whole[5:35])               # rows inside it
+        assert np.array_equal(whole[5:35], w[tokens])
+        doubled(whole, out)
+        assert np.array_equal(out, 2 * whole)
+        appy.embedding(torch.from_numpy(w), torch.from_numpy(tokens), out=torch.from_numpy(whole)[:30])      # its memory under another name
+        doubled(whole, out)
+        assert np.array_equal(out, 2 * whole) and np.array_equal(whole[:30], w[tokens])
+    finally:
+        appy.release(whole)
