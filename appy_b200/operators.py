@@ -57,7 +57,9 @@ def _through_host(fn, args, kwargs):
     from . import to_gpu
 
     def up(a):
-        return to_gpu(a) if isinstance(a, np.ndarray) or (isinstance(a, torch.Tensor) and not a.is_cuda) else a
+        if isinstance(a, np.ndarray):
+            return to_gpu(a).view(a.shape)         # which hands a single number back as an array of one
+        return to_gpu(a) if isinstance(a, torch.Tensor) and not a.is_cuda else a
 
     def up_any(a):
         return tuple(up(x) for x in a) if isinstance(a, (tuple, list)) else up(a)

@@ -196,3 +196,14 @@ def test_loops_see_what_an_operator_wrote_to_a_resident_array(rt):
         assert np.array_equal(out, 2 * whole) and np.array_equal(whole[:30], w[tokens])
     finally:
         appy.release(whole)
+
+
+def test_host_scalars_keep_their_shape(rt):
+    w = np.arange(24, dtype=np.float32).reshape(6, 4)
+    e = appy.embedding(w, np.array(3))
+    assert e.shape == (4,) and np.array_equal(e, w[3])
+    r = appy.token_logprobs(w[2], np.array(1), top=2)
+    assert r.logprobs.shape == () and r.stats.shape == (3,) and r.top_tokens.shape == (2,)
+    assert appy.token_logprobs_grad(w[2], np.array(1), r.stats, r.logprobs).shape == (4,)
+    g = appy.embedding_grad(w[0], np.array(2), 5)
+    assert g.shape == (5, 4) and np.array_equal(g[2], w[0]) and not g[[0, 1, 3, 4]].any()
