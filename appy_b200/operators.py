@@ -5,8 +5,8 @@ repeats, a scalar carried from one iteration to the next, and a reduction over (
 
 Every function launches prebuilt kernels of libappy_sm100 (include/appy_sm100.h) on torch's current stream of the
 arguments' device and returns without waiting.  Arguments are torch CUDA tensors, used in place; if the first one is
-a NumPy array or a CPU tensor, all host arrays are uploaded, and results come back as the first argument's kind, as
-with annotated loops.  Element types are float32, float16 and bfloat16; arithmetic is float32, a result is rounded
+a NumPy array or a CPU tensor, all host arrays are uploaded, and results come back as the first argument's kind, or in
+the arrays given for them, as with annotated loops.  Element types are float32, float16 and bfloat16; arithmetic is float32, a result is rounded
 once.  Token and offset arrays are int32 or int64.  Inputs may have any strides (a layout that the kernels do not read
 in place, such as a transposed last dimension, is copied first); arrays that are written need a unit last stride.
 
@@ -69,15 +69,17 @@ def _through_host(fn, args, kwargs):
         raise TypeError(f"{fn.__name__}: expected a NumPy array or a torch tensor, got {type(first).__name__}")
     dev_args, dev_kwargs = [up(a) for a in args], {k: up_any(a) for k, a in kwargs.items()}
     result = fn(*dev_args, **dev_kwargs)
-    written = {}                                   # device tensor -> the host array that the caller gave for it
+    written = {}                                   # device tensor -> the array that the caller gave for it
     for name in ("out", "last"):
         given, dev = kwargs.get(name), dev_kwargs.get(name)
         pairs = zip(given, dev) if isinstance(given, (tuple, list)) else ((given, dev),)
         for h, d in pairs:
-            if h is not None and h is not d:
+            if h is None:
+                continue
+            if h is not d:
                 (torch.from_numpy(h) if isinstance(h, np.ndarray) else h).copy_(d)
                 _touch(h)
-                written[id(d)] = h
+            written[id(d)] = h
 
     def down(t):
         if not isinstance(t, torch.Tensor):

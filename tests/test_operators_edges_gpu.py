@@ -207,3 +207,13 @@ def test_host_scalars_keep_their_shape(rt):
     assert appy.token_logprobs_grad(w[2], np.array(1), r.stats, r.logprobs).shape == (4,)
     g = appy.embedding_grad(w[0], np.array(2), 5)
     assert g.shape == (5, 4) and np.array_equal(g[2], w[0]) and not g[[0, 1, 3, 4]].any()
+
+
+def test_a_device_array_given_for_the_results_of_host_arrays_is_returned(rt):
+    w = np.arange(24, dtype=np.float32).reshape(6, 4)
+    out = torch.empty(2, 4, device="cuda")
+    assert appy.embedding(w, np.array([5, 0]), out=out) is out and np.array_equal(out.cpu().numpy(), w[[5, 0]])
+    x = w.reshape(2, 3, 4)
+    last = torch.empty(2, 4, device="cuda")
+    h, got = appy.gated_scan(x, x, last=last)
+    assert got is last and isinstance(h, np.ndarray)
