@@ -67,6 +67,11 @@ def _through_host(fn, args, kwargs):
     first = args[0]
     if not isinstance(first, (np.ndarray, torch.Tensor)):
         raise TypeError(f"{fn.__name__}: expected a NumPy array or a torch tensor, got {type(first).__name__}")
+    for name in ("out", "last"):
+        given = kwargs.get(name)
+        for h in given if isinstance(given, (tuple, list)) else (given,):
+            if isinstance(h, np.ndarray) and not h.flags.writeable:
+                raise ValueError(f"{name} is read-only")
     dev_args, dev_kwargs = [up(a) for a in args], {k: up_any(a) for k, a in kwargs.items()}
     result = fn(*dev_args, **dev_kwargs)
     written = {}                                   # device tensor -> the array that the caller gave for it
@@ -77,7 +82,10 @@ def _through_host(fn, args, kwargs):
             if h is None:
                 continue
             if h is not d:
-                (torch.from_numpy(h) if isinstance(h, np.ndarray) else h).copy_(d)
+                if isinstance(h, np.ndarray):
+                    np.copyto(h, d.cpu().numpy())
+                else:
+                    h.copy_(d)
                 _touch(h)
             written[id(d)] = h
 

@@ -217,3 +217,15 @@ def test_a_device_array_given_for_the_results_of_host_arrays_is_returned(rt):
     last = torch.empty(2, 4, device="cuda")
     h, got = appy.gated_scan(x, x, last=last)
     assert got is last and isinstance(h, np.ndarray)
+
+
+def test_read_only_host_arrays_are_not_written(rt):
+    w = np.arange(24, dtype=np.float32).reshape(6, 4)
+    out = np.zeros((2, 4), np.float32)
+    out.flags.writeable = False
+    before = rt.launch_count()
+    with pytest.raises(ValueError, match="read-only"):
+        appy.embedding(w, np.array([5, 0]), out=out)
+    assert rt.launch_count() == before and not out.any()
+    back = np.zeros((2, 4), np.float32)
+    assert appy.embedding(w, np.array([5, 0]), out=back[::-1]) is not None and np.array_equal(back, w[[0, 5]])
