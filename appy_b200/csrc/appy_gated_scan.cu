@@ -59,6 +59,8 @@ template <int V> APPY_DEV void sigmoid_pair(const float (&g)[V], Vec<V>& f, Vec<
   i = mul<V>(e, f);
 }
 
+APPY_DEV float quiet_nan() { return __int_as_float(0x7fffffff); }
+
 struct Rows {                // element (sequence s, token t, channel c) is at base + s * seq + t * row + c
   void* base;
   i64 seq, row;
@@ -203,7 +205,14 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
     const i64 n = live ? of - (k * L * C + tau0) : 0;
     return n > LT ? LT : n < 0 ? 0 : (int)n;
   };
-  bool in_time = true;                             // a wait that gave up (which cannot happen) shows as NaN
+  // A wait that gives up, which cannot happen, shows as NaN: in all that its block writes, and in the maps and states that it
+  // sends to the other blocks of its cluster from then on, and so in theirs.
+  bool in_time = true;
+  auto wait = [&](const u64* barrier, unsigned parity) { in_time = in_time && wait_full(shared_address(barrier), parity); };
+  auto meet = [&] {                                // in a cluster all threads learn whether one gave up, before they send
+    if constexpr (C > 1) in_time = __syncthreads_and(in_time);
+    else __syncthreads();
+  };
 
   // ---- reading: array 0 gate, 1 x, 2 dh, 3 h of the token before
   Pack<T, V> held[S > 1 ? 1 : NA][S > 1 ? 1 : LT];
@@ -291,7 +300,7 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
   // gates and maps of step k
   auto make = [&](i64 k, Step& st) {
     const int buf = (int)(k & 1), n = rows_left(k, len), n_before = BACK ? rows_left(k, len - 1) : n;      // one less where the sequence begins
-    if constexpr (S > 1) in_time = in_time && wait_full(shared_address(&sh.loaded[make_stage]), make_parity);
+    if constexpr (S > 1) wait(&sh.loaded[make_stage], make_parity);
     Vec<V> u[LT];
 #pragma unroll
     for (int j = 0; j < LT; ++j) {
@@ -359,6 +368,7 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
     }
     if constexpr (C > 1) {
       const unsigned full = shared_address(&sh.exchange.maps_full[buf]);
+      if (!in_time) B = quiet_nan();
       if (tid == 0) {
         expect_bytes(full, CH * 8);
         expect_bytes(shared_address(&sh.exchange.states_full[buf]), CH * 4);
@@ -373,7 +383,8 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
   auto answer = [&](i64 k) {                       // the owner's part: thread (channel, block)
     if (tid >= CH) return;
     const int buf = (int)(k & 1), ch = tid % OWN, to_rank = tid / OWN;
-    in_time = in_time && wait_full(shared_address(&sh.exchange.maps_full[buf]), (unsigned)(k >> 1) & 1);
+    wait(&sh.exchange.maps_full[buf], (unsigned)(k >> 1) & 1);
+    if (!in_time) carry = quiet_nan();
     float s = carry;
 #pragma unroll
     for (int r = 0; r < C; ++r) {
@@ -391,7 +402,7 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
     const int buf = (int)(k & 1);
     float s = carry;
     if constexpr (C > 1) {
-      in_time = in_time && wait_full(shared_address(&sh.exchange.states_full[buf]), (unsigned)(k >> 1) & 1);
+      wait(&sh.exchange.states_full[buf], (unsigned)(k >> 1) & 1);
       s = sh.exchange.state[buf][join_ch];
     }
     s = before_a * s + before_b;
@@ -404,7 +415,7 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
   };
   auto replay = [&](i64 k, const Step& st) {
     const int buf = (int)(k & 1), n = rows_left(k, len), n_before = BACK ? rows_left(k, len - 1) : n;
-    if constexpr (S > 1 && BACK) in_time = in_time && wait_full(shared_address(&sh.late_loaded[replay_stage]), replay_parity);
+    if constexpr (S > 1 && BACK) wait(&sh.late_loaded[replay_stage], replay_parity);
     float o[V];
     unpack<float, V>(ld_plain<float, V>(&sh.enter[buf][sub][pc]), o);
     Vec<V> state = vec<V>(o);
@@ -468,13 +479,13 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
         if constexpr (S == 1) fetch(k + 3);
       }
       if (C > 1 && more) join(k + 1);
-      __syncthreads();
+      meet();
       refill(k + 2);
       fetch_late(k + S);
     };
     make(0, even);
     if constexpr (S == 1) fetch(1);
-    __syncthreads();
+    meet();
     refill(0);
     send(0);
     if constexpr (C > 1) answer(0);
@@ -483,14 +494,37 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
       if constexpr (S == 1) fetch(2);
     }
     join(0);
-    __syncthreads();
+    meet();
     refill(1);
     for (i64 k = 0; k < steps; k += 2) {
       advance(k, even);
       if (k + 1 < steps) advance(k + 1, odd);
     }
   }
-  if (!in_time) carry = __int_as_float(0x7fffffff);
+  if (S > 1 || C > 1) {
+    if (__builtin_expect(__syncthreads_or(!in_time), 0)) {
+      carry = quiet_nan();
+      for (i64 k = steps - 1; k >= 0; --k) {
+        to -= to_row * L * C;
+        to_gate -= BACK ? gate_row * L * C : 0;
+        const int n = rows_left(k, len);
+        for (int j = 0; j < n; ++j)
+          for (int v = 0; v < V; ++v) {
+            reinterpret_cast<T*>(to + j * to_row)[v] = from_f32<T>(quiet_nan());
+            if (BACK) reinterpret_cast<T*>(to_gate + j * gate_row)[v] = from_f32<T>(quiet_nan());
+          }
+        // the last copies to arrive in each buffer: none outlives its block (each wait ends by itself)
+        if (S > 1 && k >= steps - S) {
+          wait_full(shared_address(&sh.loaded[k % S]), (unsigned)(k / S) & 1);
+          if (BACK) wait_full(shared_address(&sh.late_loaded[k % S]), (unsigned)(k / S) & 1);
+        }
+        if (C > 1 && k >= steps - 2) {
+          wait_full(shared_address(&sh.exchange.maps_full[k & 1]), (unsigned)(k >> 1) & 1);
+          wait_full(shared_address(&sh.exchange.states_full[k & 1]), (unsigned)(k >> 1) & 1);
+        }
+      }
+    }
+  }
   if (a.final_state && (C == 1 ? lane < WC : tid < OWN) && chan0 + carry_ch < a.width) a.final_state[seq * a.width + chan0 + carry_ch] = carry;
 }
 
