@@ -705,16 +705,6 @@ GradPlan grad_plan(i64 n, i64 rows, i64 width, int vec) {
 
 template <int ITEMS, int C> int launch_one(const OneSort& a, bool clear, cudaStream_t s) {
   const auto kernel = k_sort_clear<ITEMS, C>;
-  if (C > 8) {
-    static bool ready[16] = {false};               // per instantiation and device
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 16 || !ready[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return appy_fail_cuda(e, "embedding gradient set-up");
-      if (dev >= 0 && dev < 16) ready[dev] = true;
-    }
-  }
   cudaLaunchConfig_t cfg = {};
   // one block to an SM, and as many clusters as run at once: a GPC of 16 to 20 SMs holds one of 16 blocks, two of 8
   const int fit = std::max(2 * C, C >= 8 ? std::min(128, sm_count()) / C * C : sm_count() / C * C);
@@ -727,6 +717,19 @@ template <int ITEMS, int C> int launch_one(const OneSort& a, bool clear, cudaStr
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 1 : 0;
+  if (C > 8) {
+    static signed char fits[16] = {0};             // per instantiation and device: 0 not known yet
+    int dev = 0;
+    cudaGetDevice(&dev);
+    signed char known = dev >= 0 && dev < 16 ? fits[dev] : 0;
+    if (!known) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return appy_fail_cuda(e, "embedding gradient set-up");
+      known = cluster_fits(kernel, cfg) ? 1 : -1;
+      if (dev >= 0 && dev < 16) fits[dev] = known;
+    }
+    if (known < 0) return kNoCluster;
+  }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -858,13 +861,14 @@ int appy_embedding_grad(const void* dgrad, int dtype, int64_t ldg, const void* d
     pos[x] = reinterpret_cast<int*>(ws + p.pos_at[x]);
   }
   int* const arrived = reinterpret_cast<int*>(ws + p.arrived_at);
-  int last = 0;
+  int last = 0, rc = kNoCluster;
   if (p.cluster && n) {
     const OneSort q{dtokens, wide, (int)n, (int)rows, p.passes, p.digit_bits, key[0], pos[0], reinterpret_cast<u64*>(ws + p.between_at),
                     reinterpret_cast<int*>(ws + p.counts_at), arrived, p.counters, out_bytes, row_bytes, ld_bytes};
-    const int rc = p.items == 1 ? launch_one<1>(p.cluster, q, clear, s) : p.items == 2 ? launch_one<2>(p.cluster, q, clear, s) : launch_one<4>(p.cluster, q, clear, s);
-    if (rc) return rc;
-  } else {
+    rc = p.items == 1 ? launch_one<1>(p.cluster, q, clear, s) : p.items == 2 ? launch_one<2>(p.cluster, q, clear, s) : launch_one<4>(p.cluster, q, clear, s);
+    if (rc && rc != kNoCluster) return rc;
+  }
+  if (rc == kNoCluster) {                          // many positions, or no cluster that wide
     if (n)
       for (int pass = 0; pass < p.passes; ++pass) {
         SortPass q{pass ? nullptr : dtokens, wide, rows, key[(pass + 1) & 1], pos[(pass + 1) & 1], key[pass & 1], pos[pass & 1],

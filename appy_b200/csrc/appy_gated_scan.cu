@@ -575,15 +575,6 @@ template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, 
   a.tiles = (int)((a.width + Sh::CH - 1) / Sh::CH);
   const i64 blocks = a.sequences * a.tiles * C;
   if (blocks > 0x7fffffff) return fail_named(fn, "too many sequences for one launch");
-  static bool ready[16] = {false};                 // per instantiation and device
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 16 || !ready[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename Sh::Shared));
-    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return appy_fail_cuda(e, "gated scan set-up");
-    if (dev >= 0 && dev < 16) ready[dev] = true;
-  }
   typename std::conditional<(S > 1), Maps<BACK ? 4 : 2>, NoMaps>::type maps;
   if constexpr (S > 1) {
     const Rows* rows[4] = {&a.gate, &a.x, a.dh.base ? &a.dh : &a.gate, &a.h};
@@ -601,6 +592,18 @@ template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 1 : 0;
+  static signed char fits[16] = {0};               // per instantiation and device: 0 not known yet
+  int dev = 0;
+  cudaGetDevice(&dev);
+  signed char known = dev >= 0 && dev < 16 ? fits[dev] : 0;
+  if (!known) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename Sh::Shared));
+    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return appy_fail_cuda(e, "gated scan set-up");
+    known = C <= 8 || cluster_fits(kernel, cfg) ? 1 : -1;
+    if (dev >= 0 && dev < 16) fits[dev] = known;
+  }
+  if (known < 0) return kNoCluster;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, maps);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -627,12 +630,15 @@ template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t 
   const i64 most = a.offsets ? 12 * sms : 2 * sms;
   int c = 1;
   while (c < 16 && units * 2 * c <= most && (i64)16 * LT * c < a.tokens) c *= 2;
+  if (c == 16) {
+    const int rc = launch_c<T, 4, 8, LT, S, 128, 16, 2, BACK>(a, s);
+    if (rc != kNoCluster) return rc;
+  }
   switch (c) {
     case 1: return launch_c<T, 4, 8, LT, S, 128, 1, BACK ? (wide ? 3 : 4) : 2, BACK>(a, s);
     case 2: return launch_c<T, 4, 8, LT, S, 128, 2, 2, BACK>(a, s);
     case 4: return launch_c<T, 4, 8, LT, S, 128, 4, 2, BACK>(a, s);
-    case 8: return launch_c<T, 4, 8, LT, S, 128, 8, 2, BACK>(a, s);
-    default: return launch_c<T, 4, 8, LT, S, 128, 16, 2, BACK>(a, s);
+    default: return launch_c<T, 4, 8, LT, S, 128, 8, 2, BACK>(a, s);
   }
 }
 // Rows that TMA cannot read: the same with direct loads (8 x 2048 x 1001 bfloat16 43 / 100 us; two channels a thread, for
@@ -642,12 +648,15 @@ template <class T, bool BACK> int launch_direct(const ScanArgs& a, cudaStream_t 
   const i64 sms = sm_count(), units = a.sequences * ((a.width + 31) / 32);
   int c = 1;
   while (c < 16 && units * 2 * c <= (a.offsets ? 12 : 4) * sms && (i64)4 * LT * c < a.tokens) c *= 2;
+  if (c == 16) {
+    const int rc = launch_c<T, 1, 32, LT, 1, 128, 16, 4, BACK>(a, s);
+    if (rc != kNoCluster) return rc;
+  }
   switch (c) {
     case 1: return launch_c<T, 1, 32, LT, 1, 128, 1, 4, BACK>(a, s);
     case 2: return launch_c<T, 1, 32, LT, 1, 128, 2, 4, BACK>(a, s);
     case 4: return launch_c<T, 1, 32, LT, 1, 128, 4, 4, BACK>(a, s);
-    case 8: return launch_c<T, 1, 32, LT, 1, 128, 8, 4, BACK>(a, s);
-    default: return launch_c<T, 1, 32, LT, 1, 128, 16, 4, BACK>(a, s);
+    default: return launch_c<T, 1, 32, LT, 1, 128, 8, 4, BACK>(a, s);
   }
 }
 template <class T> int launch_token(const ScanArgs& a, cudaStream_t s) {

@@ -189,6 +189,15 @@ inline int fail_named(const char* fn, const char* what) {
   snprintf(text, sizeof text, "%s: %s", fn, what);
   return appy_fail_arg(text);
 }
+// Whether clusters as wide as `cfg` says are resident at all: 16 blocks are more than every device has to offer (one that is
+// partitioned may have fewer SMs next to one another).  Not a status of an entry: the caller takes another way.
+const int kNoCluster = -1001;
+template <class K> bool cluster_fits(K kernel, const cudaLaunchConfig_t& cfg) {
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0) return true;
+  cudaGetLastError();
+  return false;
+}
 inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 inline int element_size(int dtype) { return dtype == APPY_F32 ? 4 : (dtype == APPY_F16 || dtype == APPY_BF16) ? 2 : 0; }
 
