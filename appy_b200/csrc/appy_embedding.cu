@@ -737,13 +737,16 @@ template <int ITEMS, int C> int launch_one(const OneSort& a, bool clear, cudaStr
   }
   return finish("embedding gradient sort launch");
 }
-template <int ITEMS> int launch_one(int cluster, const OneSort& a, bool clear, cudaStream_t s) {
+// The forms that grad_plan asks for: one key a thread only in a block alone, four only in 16 blocks.
+int launch_one(int items, int cluster, const OneSort& a, bool clear, cudaStream_t s) {
+  if (items == 1) return launch_one<1, 1>(a, clear, s);
+  if (items == 4) return launch_one<4, 16>(a, clear, s);
   switch (cluster) {
-    case 1: return launch_one<ITEMS, 1>(a, clear, s);
-    case 2: return launch_one<ITEMS, 2>(a, clear, s);
-    case 4: return launch_one<ITEMS, 4>(a, clear, s);
-    case 8: return launch_one<ITEMS, 8>(a, clear, s);
-    default: return launch_one<ITEMS, 16>(a, clear, s);
+    case 1: return launch_one<2, 1>(a, clear, s);
+    case 2: return launch_one<2, 2>(a, clear, s);
+    case 4: return launch_one<2, 4>(a, clear, s);
+    case 8: return launch_one<2, 8>(a, clear, s);
+    default: return launch_one<2, 16>(a, clear, s);
   }
 }
 
@@ -865,7 +868,7 @@ int appy_embedding_grad(const void* dgrad, int dtype, int64_t ldg, const void* d
   if (p.cluster && n) {
     const OneSort q{dtokens, wide, (int)n, (int)rows, p.passes, p.digit_bits, key[0], pos[0], reinterpret_cast<u64*>(ws + p.between_at),
                     reinterpret_cast<int*>(ws + p.counts_at), arrived, p.counters, out_bytes, row_bytes, ld_bytes};
-    rc = p.items == 1 ? launch_one<1>(p.cluster, q, clear, s) : p.items == 2 ? launch_one<2>(p.cluster, q, clear, s) : launch_one<4>(p.cluster, q, clear, s);
+    rc = launch_one(p.items, p.cluster, q, clear, s);
     if (rc && rc != kNoCluster) return rc;
   }
   if (rc == kNoCluster) {                          // many positions, or no cluster that wide
