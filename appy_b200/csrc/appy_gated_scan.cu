@@ -25,8 +25,10 @@ namespace {
 using namespace appy_op;
 namespace cg = cooperative_groups;
 
-// f = sigmoid(g) and i = 1 - f, each to a few units in the last place whichever is small: with e = exp(-g),
-// f = 1 / (1 + e) and i = e f.  A gate below -87 counts as -87, so that e stays finite: f is 1.6e-38 there, not less.
+// f = sigmoid(g) and i = 1 - f: with e = exp(-g), f = 1 / (1 + e) and i = e f, so that neither is a difference.  The exponent
+// -g log2(e) is rounded once, so the smaller of the two is off by up to (1.3 |g| + 8) 2^-24 of itself, the larger by a few
+// 2^-24.  A gate below -87 counts as -87, so that e stays finite: f is 1.6e-38 there, not less.  From 87.4 on e is below the
+// normal range and counts as zero: f is 1 and i is 0.
 template <class T, int V> APPY_DEV void bounded_gate(Pack<T, V> k, float (&g)[V]) {
   if constexpr (sizeof(T) == 2 && V > 1) {         // two at a time, as they came
     typename Pack<T, V>::Bits u;

@@ -9,7 +9,7 @@ import appy_b200 as appy
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_operators_gpu import TYPES, TokenLogprobs, check_logprobs, gen, grad_reference, grad_tolerance, randn, within  # noqa: E402
+from test_operators_gpu import TYPES, U, TokenLogprobs, check_logprobs, gen, grad_reference, grad_tolerance, randn, within  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ log probabilities
@@ -164,6 +164,31 @@ def test_rows_of_no_sequence_are_cleared_for_no_sequences_too(rt, dtype):
     h, last = appy.gated_scan(x, x, offsets=offsets)
     dx, dg, d0 = appy.gated_scan_grad(x, x, x, h, offsets=offsets)
     assert not h.any() and not dx.any() and not dg.any() and last.shape == d0.shape == (0, 24)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("width", [64, 61])
+def test_small_gates_and_small_complements_are_exact_to_their_size(rt, packed, width):
+    """h = f for x = 0 and a state of one, h = 1 - f for x = 1 and no state; the same factors lead to the gradients of the
+    state and of x.  The exponent is rounded once, relative to its size: (1.3 |gate| + 8) 2^-24."""
+    at = torch.tensor([0.0, 0.5, -0.5, 5.0, -5.0, 20.0, -20.0, 50.0, -50.0, 80.0, -80.0, 87.0, -87.0, 60.3, -60.3, 33.3], device="cuda")
+    gate = at[:, None, None].expand(-1, 1, width).contiguous()
+    one, f, i = torch.ones_like(gate), torch.sigmoid(gate.double()), torch.sigmoid(-gate.double())
+    bound = (1.3 * gate.double().abs() + 8) * U
+    state = torch.ones(len(at), width, device="cuda")
+    offsets, shape = (torch.arange(len(at) + 1, device="cuda"), (len(at), width)) if packed else (None, gate.shape)
+    gate, one = gate.view(shape), one.view(shape)
+    h, last = appy.gated_scan(torch.zeros_like(one), gate, state, offsets)
+    within(h.view(f.shape), f, bound * f)
+    assert torch.equal(last, h.view(last.shape))
+    h, _ = appy.gated_scan(one, gate, None, offsets)
+    within(h.view(i.shape), i, bound * i)
+    dx, _, d0 = appy.gated_scan_grad(one, one, gate, h, state, offsets)
+    within(dx.view(i.shape), i, bound * i)
+    within(d0.view(f.shape), f, bound * f)
+    open_, _ = appy.gated_scan(one, torch.full_like(gate, 87.5), None, offsets)
+    closed, _ = appy.gated_scan(torch.zeros_like(one), torch.full_like(gate, -100.0), state, offsets)
+    assert not open_.any() and ((closed > 1.6e-38) & (closed < 1.7e-38)).all()
 
 
 # ------------------------------------------------------------------------------------------------ host arrays
