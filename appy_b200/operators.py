@@ -386,7 +386,8 @@ def gated_scan(x, gate, initial=None, offsets=None, out=None, last=None):
 def gated_scan_grad(grad, x, gate, h, initial=None, offsets=None, grad_last=None, out=None):
     """Gradients of ``gated_scan`` with respect to (x, gate, initial), given those with respect to its results.
 
-    grad: gradient of h, or None; h: the states that gated_scan returned; x, gate, initial, offsets: as given to it;
+    grad: gradient of h, or None; h: the states that gated_scan returned, of x's type (the gradient of gate takes h[t-1] - x[t]
+    from them, so in 16 bits it has their rounding beside its own); x, gate, initial, offsets: as given to it;
     grad_last: gradient of the last states, float32, or None.  out: a pair of arrays for the gradients of x and gate
     (slices of one array, for instance).  The gradient of `initial` is float32 and returned even where it was None.
     """

@@ -264,8 +264,9 @@ int appy_gated_scan(const void* dx, int64_t x_seq, int64_t x_row, const void* dg
                     int64_t gate_row, int dtype, const void* doffsets, int offsets_dtype, int64_t sequences,
                     int64_t tokens, int64_t width, const float* dinitial, void* dh, int64_t h_seq, int64_t h_row,
                     float* dlast, int fill, void* stream);
-/* Its gradient: dh is the recurrence's result, ddh the gradient with respect to it (NULL: zeros), dgrad_last that with
- * respect to the last state (NULL: zeros); results are the gradients of x, gate and the initial state (NULL: not wanted). */
+/* Its gradient: dh is the recurrence's result (rounded to dtype, as it is; h[t-1] - x[t] is taken from it), ddh the
+ * gradient with respect to it (NULL: zeros), dgrad_last that with respect to the last state (NULL: zeros); results are
+ * the gradients of x, gate and the initial state (NULL: not wanted). */
 int appy_gated_scan_grad(const void* ddh, int64_t dh_seq, int64_t dh_row, const void* dx, int64_t x_seq,
                          int64_t x_row, const void* dgate, int64_t gate_seq, int64_t gate_row, const void* dh,
                          int64_t h_seq, int64_t h_row, int dtype, const void* doffsets, int offsets_dtype,
