@@ -499,7 +499,9 @@ __device__ __noinline__ void hand_in(const SumArgs& a, O* out, int share, int co
 }
 
 // A warp takes one share and 32 packs of columns, kSumAhead rows in flight before it adds up the kSumAhead before
-// them: 32 warps to an SM with 8 rows of 512 bytes each keep 128 KB in flight.
+// them: 24 warps to an SM with 4 to 8 rows of 512 bytes each keep 48 to 96 KB in flight.  At 80 registers the 16-bit packs
+// spill 108 bytes.  Two blocks to an SM with 128 registers, which spill nothing: 51 us for 53 (16384 x 4096 bfloat16 into 600
+// rows) but 64 for 60 (5003 x 769 float32).
 template <class T, class O, int V>
 __global__ void __launch_bounds__(kSumBlock, 3) k_sum_rows(const __grid_constant__ SumArgs a, const T* __restrict__ g, O* __restrict__ out) {
   constexpr int U = kSumAhead;

@@ -12,7 +12,7 @@
 //   mu[t] = f[t] * lam[t],  dx[t] = (1 - f[t]) * lam[t],  dgate[t] = lam[t] * (h[t-1] - x[t]) * f[t] * (1 - f[t]),
 // mu past the last token is the gradient of the last state, mu[0] that of the initial one.  h[t-1] is read as the forward pass
 // left it, rounded to the type of x: half a step of it in 16 bits is the largest error of dgate, about that of rounding dgate
-// itself (8 x 2048 x 2048 bfloat16: off by 0.0018 of its size, 0.0017 with float32 states).  The states in float32 would cost a
+// itself (bfloat16: off by 0.0018 of its size, 0.0016 with float32 states).  The states in float32 would cost a
 // third more bytes in the forward pass and a sixth more in this one.
 //
 // A block takes 64 or 32 channels of one sequence and walks along it; with few sequences and channels a cluster of
@@ -625,7 +625,7 @@ template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, 
 //     46 us; the first variant 53 us), gradient 4 tokens per thread and four blocks (73 us; the first variant 94 us);
 //   fewer than two 32-channel blocks per SM: clusters along the tokens, as many blocks as keep to two per SM, which
 //     is where all clusters run at once (65536 x 1024: 8 blocks 106 us, 16 blocks 160 us, one block 493 us);
-//     packed sequences, whose lengths are uneven, up to six per SM (37 sequences of 0 to 8000 tokens of 648 float32
+//     packed sequences, whose lengths are uneven, up to twelve per SM (37 sequences of 0 to 8000 tokens of 648 float32
 //     channels: two blocks 85 / 153 us, one 85 / 176 us).
 template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t s) {
   constexpr bool wide = sizeof(T) == 4;
@@ -646,8 +646,12 @@ template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t 
     default: return launch_c<T, 4, 8, LT, S, 128, 8, 2, BACK>(a, s);
   }
 }
-// Rows that TMA cannot read: the same with direct loads (8 x 2048 x 1001 bfloat16 43 / 100 us; two channels a thread, for
-// packed arithmetic, 72 / 177 us: the loads are what takes the time).
+// Rows that TMA cannot read: the same with direct loads (two channels a thread, for packed arithmetic, 72 / 177 us for
+// 8 x 2048 x 1001 bfloat16: the loads are what takes the time).  As many blocks to a cluster as keep to four per SM, for packed
+// sequences, whose lengths are uneven, to twelve.  Times for 1, 2, 4 blocks, the chosen one marked; bfloat16:
+//   8 x 2048 x 1001: 56, 46*, 48 / 137, 101*, 104 us;  16 x 2048 x 1001: 68*, 80, 87 / 169*, 182, 191;
+//   2 x 8192 x 1001: 66 / 152 with 4, 49* / 103* with 8, 65 / 138 with 16;
+//   packed, 37 sequences of 1500 tokens of 651 channels: 146, 119*, 109 / 373, 274*, 236;  200 of 150 of 1001: 76*, 131 / 161*, 219.
 template <class T, bool BACK> int launch_direct(const ScanArgs& a, cudaStream_t s) {
   constexpr int LT = BACK ? 4 : 8;
   const i64 sms = sm_count(), units = a.sequences * ((a.width + 31) / 32);
