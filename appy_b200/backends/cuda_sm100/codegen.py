@@ -1196,7 +1196,7 @@ def touch(*arrays):
 def touch_bytes(lo: int, hi: int) -> None:
     """Host memory in [lo, hi) was written: `touch` for every resident array that has part of it, by whatever name it
     was written."""
-    for p, st in _resident.items():
+    for p, st in list(_resident.items()):      # an entry goes with its array, at any time
         if p < hi and lo < p + st[0]:
             st[1] = False
 
