@@ -41,6 +41,20 @@ def test_token_logprobs_masked_by_large_finite_values(rt, dtype, mask, temperatu
     check_logprobs(torch.cat([logits] * 40), torch.cat([tokens] * 40), temperature, 5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1e-4, 1e4])
+@pytest.mark.parametrize("std", [1.0, 100.0, 1e4])
+def test_token_logprobs_at_both_ends_of_the_temperature(rt, dtype, temperature, std):
+    for cols in (9, 1001, 20000):
+        logits = randn(5, cols, dtype=dtype, seed=cols, std=std)
+        logits[1] += 3 * std
+        logits[2] -= 3 * std
+        logits[3, ::3] = -math.inf
+        tokens = logits.argmax(-1)
+        tokens[4] = cols - 1
+        check_logprobs(logits, tokens, temperature, 5)
+
+
 def test_results_of_log_probabilities_are_arrays_of_their_own(rt):
     logits, tokens = randn(6, 50, seed=1).requires_grad_(), torch.arange(6, device="cuda")
     lp, entropy = TokenLogprobs.apply(logits, tokens)
