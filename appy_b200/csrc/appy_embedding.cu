@@ -11,8 +11,8 @@
 // in the workspace, and the warp that hands in the last piece folds them in share order.  Sums are float32
 // throughout, rounded once.
 //
-// Up to 65536 positions one cluster of blocks sorts, and the blocks beside it clear the rows without tokens meanwhile:
-// most of the gradient's bytes are those zeros, so the sort costs next to nothing.
+// Up to 65536 positions one cluster of blocks sorts, and the blocks beside it clear the rows without tokens meanwhile: with a
+// large vocabulary most of the gradient's bytes are those zeros, and the sort is hidden behind them.
 #include <cooperative_groups.h>
 
 #include "operators.cuh"
@@ -28,7 +28,7 @@ APPY_DEV i64 token_of(const void* tokens, bool wide, i64 n) {
 
 // ------------------------------------------------------------------------------------------------ lookup
 // Rows of at least 32 packs: a warp takes a stretch of one row, so that no pack needs an index of its own (65536 rows
-// of 4096 bfloat16 121 us; the flat form, at 118 instructions per 32 packs, four fifths of all issue slots, 144).  Shorter
+// of 4096 bfloat16 117 us; the flat form, at 118 instructions per 32 packs, four fifths of all issue slots, 144).  Shorter
 // rows: flat over the packs of the output, pack i of row i / per_row; neighbouring threads read one row, so token
 // loads are broadcasts.
 const int kLookupBlock = 256;

@@ -624,9 +624,9 @@ template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, 
 //   fewer: 32-channel blocks, twice as many; forward 8 tokens per thread and two blocks to an SM (8 x 2048 x 2048:
 //     46 us; the first variant 53 us), gradient 4 tokens per thread and four blocks (73 us; the first variant 94 us);
 //   fewer than two 32-channel blocks per SM: clusters along the tokens, as many blocks as keep to two per SM, which
-//     is where all clusters run at once (65536 x 1024: 8 blocks 106 us, 16 blocks 160 us, one block 493 us);
+//     is where all clusters run at once (65536 x 1024: 8 blocks 108 us, 16 blocks 160 us, one block 493 us);
 //     packed sequences, whose lengths are uneven, up to twelve per SM (37 sequences of 0 to 8000 tokens of 648 float32
-//     channels: two blocks 85 / 153 us, one 85 / 176 us).
+//     channels: two blocks 86 / 154 us, one 85 / 176 us).
 template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t s) {
   constexpr bool wide = sizeof(T) == 4;
   constexpr int S = wide || BACK ? 2 : 4, LT = BACK ? 4 : 8;
