@@ -101,9 +101,9 @@ template <class T, int V> APPY_DEV void clear_rows(const Rows& r, i64 lo, i64 hi
 }
 
 APPY_DEV unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-// The wait suspends the warp for up to a microsecond at a time; false: it gave up after about a second.
+// Each try suspends the warp for up to about 4 us; false: it gave up after about a second.
 APPY_DEV bool wait_full(unsigned barrier, unsigned parity) {
-  for (unsigned tries = 0; tries < (1u << 20); ++tries) {
+  for (unsigned tries = 0; tries < (1u << 18); ++tries) {
     unsigned done;
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
                  : "=r"(done) : "r"(barrier), "r"(parity), "r"(1000u) : "memory");
@@ -210,8 +210,8 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
     const i64 n = live ? of - (k * L * C + tau0) : 0;
     return n > LT ? LT : n < 0 ? 0 : (int)n;
   };
-  // A wait that gives up, which cannot happen, shows as NaN: in all that its block writes, and in the maps and states that it
-  // sends to the other blocks of its cluster from then on, and so in theirs.
+  // A wait that gives up, which cannot happen, shows as NaN in all that its block writes.  In a cluster the block stops with the
+  // step, so the others, which wait for its next message, give up too, and none of them leaves before the rest.
   bool in_time = true;
   auto wait = [&](const u64* barrier, unsigned parity) { in_time = in_time && wait_full(shared_address(barrier), parity); };
   auto meet = [&] {                                // in a cluster all threads learn whether one gave up, before they send
@@ -373,7 +373,6 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
     }
     if constexpr (C > 1) {
       const unsigned full = shared_address(&sh.exchange.maps_full[buf]);
-      if (!in_time) B = quiet_nan();
       if (tid == 0) {
         expect_bytes(full, CH * 8);
         expect_bytes(shared_address(&sh.exchange.states_full[buf]), CH * 4);
@@ -389,7 +388,7 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
     if (tid >= CH) return;
     const int buf = (int)(k & 1), ch = tid % OWN, to_rank = tid / OWN;
     wait(&sh.exchange.maps_full[buf], (unsigned)(k >> 1) & 1);
-    if (!in_time) carry = quiet_nan();
+    if (!in_time) return;
     float s = carry;
 #pragma unroll
     for (int r = 0; r < C; ++r) {
@@ -501,33 +500,28 @@ k_scan(const ScanArgs a, const __grid_constant__ typename std::conditional<(S > 
     join(0);
     meet();
     refill(1);
-    for (i64 k = 0; k < steps; k += 2) {
+    for (i64 k = 0; k < steps && (C == 1 || in_time); k += 2) {
       advance(k, even);
-      if (k + 1 < steps) advance(k + 1, odd);
+      if (k + 1 < steps && (C == 1 || in_time)) advance(k + 1, odd);
     }
   }
   if (S > 1 || C > 1) {
     if (__builtin_expect(__syncthreads_or(!in_time), 0)) {
       carry = quiet_nan();
-      for (i64 k = steps - 1; k >= 0; --k) {
-        to -= to_row * L * C;
-        to_gate -= BACK ? gate_row * L * C : 0;
+      to = reinterpret_cast<char*>(row_ptr<T>(BACK ? a.dx : a.h, seq_at, first, t0, col));
+      if (BACK) to_gate = reinterpret_cast<char*>(row_ptr<T>(a.dgate, seq_at, first, t0, col));
+      for (i64 k = 0; k < steps; ++k) {
         const int n = rows_left(k, len);
         for (int j = 0; j < n; ++j)
           for (int v = 0; v < V; ++v) {
             reinterpret_cast<T*>(to + j * to_row)[v] = from_f32<T>(quiet_nan());
             if (BACK) reinterpret_cast<T*>(to_gate + j * gate_row)[v] = from_f32<T>(quiet_nan());
           }
-        // the last copies to arrive in each buffer: none outlives its block (each wait ends by itself)
-        if (S > 1 && k >= steps - S) {
-          wait_full(shared_address(&sh.loaded[k % S]), (unsigned)(k / S) & 1);
-          if (BACK) wait_full(shared_address(&sh.late_loaded[k % S]), (unsigned)(k / S) & 1);
-        }
-        if (C > 1 && k >= steps - 2) {
-          wait_full(shared_address(&sh.exchange.maps_full[k & 1]), (unsigned)(k >> 1) & 1);
-          wait_full(shared_address(&sh.exchange.states_full[k & 1]), (unsigned)(k >> 1) & 1);
-        }
+        to += to_row * L * C;
+        to_gate += BACK ? gate_row * L * C : 0;
       }
+      if constexpr (C > 1) cg::this_cluster().sync();
+      for (int x = 0; x < 10; ++x) __nanosleep(100000);          // for what is on its way to this block
     }
   }
   if (a.final_state && (C == 1 ? lane < WC : tid < OWN) && chan0 + carry_ch < a.width) a.final_state[seq * a.width + chan0 + carry_ch] = carry;
@@ -622,11 +616,11 @@ template <class T, int V, int CP, int LT, int S, int NT, int C, int MIN_BLOCKS, 
 //     (64 x 512 x 2048: 71 us; 32-channel blocks of 8 tokens per thread 96 us), and short sequences (16 x 100 x 2048:
 //     8 / 12 us; the others 12 / 14 us);
 //   fewer: 32-channel blocks, twice as many; forward 8 tokens per thread and two blocks to an SM (8 x 2048 x 2048:
-//     46 us; the first variant 53 us), gradient 4 tokens per thread and four blocks (73 us; the first variant 94 us);
+//     47 us; the first variant 53 us), gradient 4 tokens per thread and four blocks (73 us; the first variant 94 us);
 //   fewer than two 32-channel blocks per SM: clusters along the tokens, as many blocks as keep to two per SM, which
-//     is where all clusters run at once (65536 x 1024: 8 blocks 108 us, 16 blocks 160 us, one block 493 us);
+//     is where all clusters run at once (65536 x 1024: 8 blocks 109 us, 16 blocks 160 us, one block 493 us);
 //     packed sequences, whose lengths are uneven, up to twelve per SM (37 sequences of 0 to 8000 tokens of 648 float32
-//     channels: two blocks 86 / 154 us, one 85 / 176 us).
+//     channels: two blocks 87 / 154 us, one 85 / 176 us).
 template <class T, bool BACK> int launch_packed(const ScanArgs& a, cudaStream_t s) {
   constexpr bool wide = sizeof(T) == 4;
   constexpr int S = wide || BACK ? 2 : 4, LT = BACK ? 4 : 8;
