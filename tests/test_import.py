@@ -1,4 +1,5 @@
 """What importing the package brings along."""
+import os
 import subprocess
 import sys
 
@@ -15,7 +16,8 @@ sys.meta_path.insert(0, NoTorch())
 
 
 def run(code):
-    return subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(appy.__file__)))
+    return subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=root)
 
 
 def test_a_star_import_needs_no_torch():
